@@ -158,6 +158,9 @@ namespace nhb {
 		// cleaned it) and the k tile of the scores issued behind it.  The issuing thread must not wait often: while products stream
 		// their operands from shared memory, a look at a barrier there takes some 250 cycles.
 		constexpr int P_ARRIVALS = 8 + 8 + 2;
+		// A slot of the ring is free once the products that read it have run and both watching warps have seen its tile: they follow
+		// every phase of every slot by its parity, and a warp that comes after the slot's next tile would wait for a phase that has passed.
+		constexpr int EMPTY_ARRIVALS = 1 + 2;
 		__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, int n) {
 			asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 		}
@@ -294,7 +297,7 @@ namespace nhb {
 			if (tid == 0) {
 				for (int s = 0; s < NST; ++s) {
 					mbar_init(&hd->full[s], 1);
-					mbar_init(&hd->empty[s], 1);
+					mbar_init(&hd->empty[s], EMPTY_ARRIVALS);
 				}
 				for (int b = 0; b < NS; ++b) {
 					mbar_init(&hd->s_full[b], 1);
@@ -540,10 +543,13 @@ namespace nhb {
 				} else {
 					// ---------------- the ring's tiles, in order; v tiles that not every row sees whole are cleaned ----------------
 					bool odd = false, ok = true;
-					int seen = 0;// positions of the ring's order that have landed: every phase of every slot is followed
+					int seen = 0;// positions of the ring's order that have landed; the slot is not filled again before its arrival here
 					const auto see = [&](int at) {
-						for (; seen <= at && ok; ++seen)
-							ok = mbar_wait(&hd->full[seen % NST], (seen / NST) & 1);
+						for (; seen <= at && ok; ++seen) {
+							ok = __all_sync(0xffffffffu, mbar_wait(&hd->full[seen % NST], (seen / NST) & 1));
+							if (ok && lane == 0)
+								mbar_arrive(&hd->empty[seen % NST]);
+						}
 					};
 					for (int t = 0; t < steps && ok; ++t) {
 						const int j = two ? t >> 1 : t, at = v_at(j, n_tiles, ahead), s = at % NST;
@@ -591,7 +597,7 @@ namespace nhb {
 						if (t + NS < steps)
 							see(k_at(two ? (t + NS) >> 1 : t + NS, ahead));
 						if (t >= NS && ok)// not ahead of the buffer's step before: an arrival would count for that one
-							ok = mbar_wait(&hd->p_full[t % NS], (t / NS - 1) & 1);
+							ok = __all_sync(0xffffffffu, mbar_wait(&hd->p_full[t % NS], (t / NS - 1) & 1));
 						__syncwarp();
 						if (lane == 0)// nothing was multiplied before step 0: no product to be taken
 							mbar_arrive_n(&hd->p_full[t % NS], t == 0 && warp == 2 ? 1 + 8 : 1);

@@ -1,0 +1,179 @@
+"""How the warps of the attention kernels hand tiles to one another, on a model of their barriers (no GPU): whatever warp is late, every tile
+is read in its own phase, nothing is overwritten while it is in use and every wait ends.  The numbers of arrivals come from the source."""
+import os
+import re
+
+import pytest
+
+from tests.ring_model import Bar, Meeting, Run
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "nihilus_b200", "csrc")
+
+
+def _source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return f.read()
+
+
+def _number(source, name, default=None):
+    m = re.search(r"constexpr int %s\s*=\s*([0-9 +]+);" % name, source)
+    return sum(int(x) for x in m.group(1).split("+")) if m else default
+
+
+# ---- prompts: copies, products, two warps that watch the ring, sixteen of the softmax ----
+
+KB = 1024
+
+
+def _prompt_config(d, bf16, two):
+    """(slots of the ring, score buffers) as attn_prompt.cu has them."""
+    parts, buffers = (3, 2) if bf16 else (2, 3)
+    queries = parts * (2 if two else 1) * 128 * d * 2
+    return min(8, (224 * KB - queries) // (128 * d * 2)), buffers
+
+
+CONFIGS = [(d, bf16, two) for d in (64, 128) for bf16 in (False, True) for two in (False, True) if not (bf16 and d == 128 and two)]
+
+
+def k_at(j, ahead):
+    return j + max(0, j - ahead + 1)
+
+
+def v_at(j, n, ahead):
+    return j + min(ahead + j, n)
+
+
+def prompt_run(config, n, **schedule):
+    """A CTA over n key tiles."""
+    two = config[2]
+    slots, buffers = _prompt_config(*config)
+    source = _source("attn_prompt.cu")
+    empty_arrivals = _number(source, "EMPTY_ARRIVALS", 1)
+    run = Run(**schedule)
+    ahead, steps = (buffers - 1, 2 * n) if two else (buffers, n)
+    full, empty = [Bar(1) for _ in range(slots)], [Bar(empty_arrivals) for _ in range(slots)]
+    s_full, p_full = [Bar(1) for _ in range(buffers)], [Bar(_number(source, "P_ARRIVALS")) for _ in range(buffers)]
+    o_full, q_full = [Bar(1), Bar(1)], Bar(16)
+    softmax, chains, end = Meeting(16), [Meeting(8), Meeting(8)], Meeting(20)
+    content, scores_of, product = [None] * slots, [None] * buffers, [None]
+    untaken, left = [0], [0] * buffers  # warps that have yet to take the product; warps that have left their weights over the scores
+
+    def land(slot, tile):
+        content[slot] = tile
+
+    def copies():
+        kj = vj = 0
+        for at in range(2 * n):
+            is_v = not (kj < n and kj < ahead + vj)
+            tile = ("v", vj) if is_v else ("k", kj)
+            kj, vj = kj + (not is_v), vj + is_v
+            assert at == (v_at(tile[1], n, ahead) if is_v else k_at(tile[1], ahead))
+            s = at % slots
+            if not (yield empty[s], ((at // slots) & 1) ^ 1):
+                break
+            content[s] = None
+            full[s].arrive(tx=1)
+            run.copies.append((full[s], lambda s=s, tile=tile: land(s, tile)))
+        yield end, end.join()
+
+    def use(slot, tile, t, buf, is_scores):
+        run.check(content[slot] == tile, "a product reads", content[slot], "for", tile)
+        if is_scores:
+            scores_of[buf], left[buf] = t, 0
+        else:
+            run.check(scores_of[buf] == t and left[buf] == 8, "weights of", left[buf], "warps of", scores_of[buf], "for", t)
+            run.check(untaken[0] == 0, "a product is overwritten")
+            product[0], untaken[0] = t, 8
+
+    def products():
+        def issue(t, is_scores):
+            j, buf = (t >> 1 if two else t), t % buffers
+            s = (k_at(j, ahead) if is_scores else v_at(j, n, ahead)) % slots
+            run.products.append(lambda: use(s, ("k" if is_scores else "v", j), t, buf, is_scores))
+            run.products.append(lambda: (s_full[buf] if is_scores else o_full[t & 1]).arrive())
+            if not two or t & 1:
+                run.products.append(lambda: empty[s].arrive())
+
+        ok = yield q_full, 0
+        for t in range(min(buffers, steps)):
+            if not ok:
+                break
+            at = k_at(t >> 1 if two else t, ahead)
+            ok = yield full[at % slots], (at // slots) & 1
+            if ok:
+                issue(t, True)
+        for t in range(steps):
+            if not ok:
+                break
+            ok = yield p_full[t % buffers], (t // buffers) & 1
+            if not ok:
+                break
+            issue(t, False)
+            if t + buffers < steps:
+                issue(t + buffers, True)
+        yield end, end.join()
+
+    def watcher(first):
+        seen, ok = 0, True
+        for t in range(steps):
+            j = t >> 1 if two else t
+            at = v_at(j, n, ahead)
+            last = k_at((t + buffers) >> 1 if two else t + buffers, ahead) if t + buffers < steps else -1
+            for target in (at, last):
+                while seen <= target and ok:
+                    ok = yield full[seen % slots], (seen // slots) & 1
+                    if ok and empty_arrivals > 1:
+                        empty[seen % slots].arrive()
+                    seen += 1
+                if target == at and ok:
+                    run.check(content[at % slots] == ("v", j), "a watcher cleans", content[at % slots], "for", j)
+            if t >= buffers and ok:
+                ok = yield p_full[t % buffers], (t // buffers - 1) & 1
+            if not ok:
+                break
+            p_full[t % buffers].arrive(1 + 8 if t == 0 and first else 1)
+        yield end, end.join()
+
+    def weights(chain):
+        q_full.arrive()
+        yield softmax, softmax.join()
+        yield softmax, softmax.join()
+        ok, use_ = True, 0
+        for _ in range(0 if two else chain, n, 1 if two else 2):
+            t = 2 * use_ + chain
+            ok = ok and (yield s_full[t % buffers], (t // buffers) & 1)
+            run.check(scores_of[t % buffers] == t, "scores", scores_of[t % buffers], "for", t)
+            yield chains[chain], chains[chain].join()
+            left[t % buffers] += 1
+            yield None
+            p_full[t % buffers].arrive()
+            ok = ok and (yield o_full[chain], use_ & 1)
+            run.check(product[0] == t, "product", product[0], "for", t)
+            untaken[0] -= 1
+            yield None
+            if t + 1 < steps:
+                p_full[(t + 1) % buffers].arrive()
+            use_ += 1
+        yield softmax, softmax.join()
+        yield end, end.join()
+
+    run.warps = {"copies of tiles": copies(), "products of tiles": products(), "watcher 2": watcher(True), "watcher 3": watcher(False)}
+    for w in range(16):
+        run.warps[f"softmax {w}"] = weights(w >> 3)
+    run.go()
+
+
+WARPS = ["copies of tiles", "products of tiles", "watcher 2", "watcher 3", "softmax 0", "softmax 9", "copies", "products"]
+
+
+@pytest.mark.parametrize("config", CONFIGS)
+def test_prompt_ring_holds_whichever_warp_is_late(config):
+    for n in (1, 2, 3, 4, 6, 9):
+        for seed in range(2):
+            prompt_run(config, n, seed=seed)
+        for late in [(w,) for w in WARPS] + [("watcher 2", "watcher 3")]:
+            prompt_run(config, n, seed=7, late=late)
+    for n in (2, 6):
+        for warp in WARPS[:6]:
+            for turns in range(0, 14):
+                prompt_run(config, n, seed=turns, held=(warp, turns))
