@@ -17,7 +17,8 @@
 //   warps 2, 3   watch the ring, and clean v tiles that some row may see only in part: rows past the end become zero, and so do
 //                infinities and NaN (0 * inf would reach rows that may not see them; rows that may get them back at the end)
 //   warps 4-19   softmax, two threads per row, and the running sums (head_dim / 2 registers each)
-// Every wait is bounded; one that runs out is recorded for the host.
+// Every wait is bounded; one that runs out is recorded for the host.  A warp whose wait ran out arrives nowhere any more, so that what waits for
+// it stops too, and the block ends only after its copies and products.
 //
 // B200, f16, 32 heads of 128 on 8: 8192 tokens 863 us (637 TFLOP/s of the formula, 1274 on the tensor cores; about 1.0 ms once the
 // power limit has brought the clock down), 2048 tokens 96 us, 77 tokens 15.5 us.  A step (one chain's scores and P V, 32
@@ -63,6 +64,7 @@ namespace nhb {
 			uint64_t s_full[3], p_full[3];// per score buffer
 			uint64_t o_full[2];// per chain
 			uint64_t q_full;
+			uint64_t drain;// all products have run
 			union {
 				float back[2 * TILE];// before the first tile: what undoes a row's scaling, times scale log2(e)
 				float half[2][2][TILE];// per chain and half of the columns: a row's largest score of the tile; at the end its sum
@@ -306,6 +308,7 @@ namespace nhb {
 				mbar_init(&hd->o_full[0], 1);
 				mbar_init(&hd->o_full[1], 1);
 				mbar_init(&hd->q_full, 16);
+				mbar_init(&hd->drain, 1);
 				fence_mbar_init();
 				hd->odd	  = 0;
 				hd->entry = -1;
@@ -443,6 +446,7 @@ namespace nhb {
 					int page[2] = { 0, 0 }, page0[2] = { -64, -64 };
 					const int loads	 = 2 * n_tiles;
 					bool ok			 = true;
+					int issued		 = 0;
 					int kj = 0, vj = 0;
 					for (int at = 0; at < loads && ok; ++at) {
 						const int is_v = !(kj < n_tiles && kj < ahead + vj);
@@ -483,16 +487,24 @@ namespace nhb {
 						if (b < boxes && ok)
 							tma_load_2d(smem_u32(ring) + s * SLOT + c * PANEL + b * box * 128, is_v ? &map_v : &map_k, c * 64,
 								((pg * p.c.kv_heads + kvh) << p.c.page_shift) + (k & (p.c.page_tokens - 1)), &hd->full[s]);
+						issued += ok;
 						__syncwarp();
 					}
+					// the last copy into each slot has landed before the block ends
+					if (lane == 0)
+						for (int at = max(0, issued - NST); at < issued; ++at)
+							if (!mbar_wait(&hd->full[at % NST], (at / NST) & 1))
+								atomicExch(p.c.status, DEV_TIMEOUT_DRAIN);
 				} else if (warp == 1) {
 					// ---------------- products ----------------
 					if (elect_one() && n_tiles > 0) {
 						constexpr uint32_t id_s = instr_desc(KT, BF16, false), id_o = instr_desc(D, BF16, true);
 						const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(base);
 						bool ok = mbar_wait(&hd->q_full, 0);
+						// whether the slot of this position of the ring's order is filled once more: nobody waits for it otherwise
+						const auto again  = [&](int pos) { return pos + NST < 2 * n_tiles; };
 						const auto scores = [&](int t) {
-							const int c = t & 1, j = two ? t >> 1 : t, buf = t % NS, s = k_at(j, ahead) % NST;
+							const int c = t & 1, j = two ? t >> 1 : t, buf = t % NS, pos = k_at(j, ahead), s = pos % NST;
 							const uint32_t d  = tmem + COL_S + buf * KT;
 							const uint32_t kd = desc_lo(ring_a + s * SLOT, 16);
 #pragma unroll
@@ -503,7 +515,7 @@ namespace nhb {
 									mma_ss(d, qd + (k >> 2) * ((TILE * 128) >> 4) + (k & 3) * 2, DESC_HI, kd + (k >> 2) * (PANEL >> 4) + (k & 3) * 2, DESC_HI, id_s, part < PARTS - 1 || k > 0);
 							}
 							umma_commit_a(smem_u32(&hd->s_full[buf]));
-							if (!two || c == 1)
+							if ((!two || c == 1) && again(pos))
 								umma_commit_a(smem_u32(&hd->empty[s]));
 						};
 						// step t is chain t & 1; its scores are NS steps ahead, so their buffer is free once P V of step t - NS has been issued
@@ -515,7 +527,7 @@ namespace nhb {
 								scores(t);
 						}
 						for (int t = 0; t < steps && ok; ++t) {
-							const int c = t & 1, j = two ? t >> 1 : t, buf = t % NS, s = v_at(j, n_tiles, ahead) % NST;
+							const int c = t & 1, j = two ? t >> 1 : t, buf = t % NS, pos = v_at(j, n_tiles, ahead), s = pos % NST;
 							ok = mbar_wait(&hd->p_full[buf], (t / NS) & 1);
 							if (!ok)
 								break;
@@ -532,13 +544,16 @@ namespace nhb {
 									mma_ts(d, w, vd + k * (2048 >> 4), DESC_HI, id_o, part < PARTS - 1 || k > 0);
 								}
 							umma_commit_a(smem_u32(&hd->o_full[c]));
-							if (!two || c == 1)
+							if ((!two || c == 1) && again(pos))
 								umma_commit_a(smem_u32(&hd->empty[s]));
 							if (t + NS < steps)
 								scores(t + NS);
 						}
 						if (!ok)
 							atomicExch(p.c.status, DEV_TIMEOUT_MMA);
+						umma_commit_a(smem_u32(&hd->drain));
+						if (!mbar_wait(&hd->drain, 0))
+							atomicExch(p.c.status, DEV_TIMEOUT_DRAIN);
 					}
 				} else {
 					// ---------------- the ring's tiles, in order; v tiles that not every row sees whole are cleaned ----------------
@@ -599,7 +614,7 @@ namespace nhb {
 						if (t >= NS && ok)// not ahead of the buffer's step before: an arrival would count for that one
 							ok = __all_sync(0xffffffffu, mbar_wait(&hd->p_full[t % NS], (t / NS - 1) & 1));
 						__syncwarp();
-						if (lane == 0)// nothing was multiplied before step 0: no product to be taken
+						if (lane == 0 && ok)// nothing was multiplied before step 0: no product to be taken
 							mbar_arrive_n(&hd->p_full[t % NS], t == 0 && warp == 2 ? 1 + 8 : 1);
 					}
 					if (!ok && lane == 0)
@@ -691,7 +706,7 @@ namespace nhb {
 					}
 					tc_fence_before();
 					__syncwarp();
-					if (lane == 0 && 2 * n + chain + 1 < steps)
+					if (lane == 0 && ok && 2 * n + chain + 1 < steps)
 						mbar_arrive(&hd->p_full[(2 * n + chain + 1) % NS]);
 				};
 				for (int j = two ? 0 : chain; j < n_tiles; j += two ? 1 : 2, ++use) {
@@ -712,12 +727,12 @@ namespace nhb {
 					tmem_st_wait();
 					tc_fence_before();
 					__syncwarp();
-					if (lane == 0)
+					if (lane == 0 && ok)
 						mbar_arrive(&hd->p_full[buf]);
 					l = fmaf(l, keep, sum);
 					add_product(use, keep);
 				}
-				if (!ok && lane == 0)
+				if (!ok)
 					atomicExch(p.c.status, DEV_TIMEOUT_MMA);
 				tc_fence_before();
 				softmax_barrier();// all products have run, all maxima are read

@@ -1,7 +1,7 @@
 """Barriers, copies and products of a kernel whose warps hand tiles to one another, run step by step on the host under any schedule.
 
 A warp is a generator.  It yields a barrier and a parity to wait for (and is sent True, or False where the model lets the wait run
-out) or None to let others go first.  What runs beside the warps -- copies, which land in any order, and products, which run in the order in
+out; a third value True: it may not) or None to let others go first.  What runs beside the warps -- copies, which land in any order, and products, which run in the order in
 which they were issued -- lies in `copies` and `products`."""
 import random
 
@@ -84,7 +84,7 @@ class Run:
         freed = self.held is None
         while waits:
             ready = [w for w, x in waits.items() if x is None or x[0].passed(x[1])]
-            timed = [w for w, x in waits.items() if x is not None and isinstance(x[0], Bar) and not x[0].passed(x[1])]
+            timed = [w for w, x in waits.items() if x is not None and isinstance(x[0], Bar) and len(x) == 2 and not x[0].passed(x[1])]
             most = [w for w in ready if w not in self.late and (freed or w != self.held[0] or turns[w] < self.held[1])]
             beside = [k for k in ("copies", "products") if getattr(self, k) and k not in self.late]
             if self.give_up and timed and self.r.random() < self.give_up:
@@ -92,6 +92,8 @@ class Run:
                 self.failed = True
             elif most or beside:
                 w, answer = self.r.choice(most + beside * 3), True
+            elif self.failed and timed and self.r.random() < 0.5:
+                w, answer = self.r.choice(timed), False  # one warp gives up after the other while what is late still runs
             elif self.copies or self.products:
                 w, answer = ("copies" if self.copies else "products"), True
             elif ready:
@@ -110,5 +112,5 @@ class Run:
                     waits[w] = self.warps[w].send(answer if waits[w] is not None else None)
                 except StopIteration:
                     del waits[w]
-        if self.copies:
-            raise Fault(("the block ends with copies in flight", len(self.copies)))
+        if self.copies or self.products:
+            raise Fault(("the block ends with work in flight", len(self.copies), len(self.products)))

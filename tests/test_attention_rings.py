@@ -20,6 +20,14 @@ def _number(source, name, default=None):
     return sum(int(x) for x in m.group(1).split("+")) if m else default
 
 
+def _only_if_ok(source, arrival):
+    """Whether every such arrival stands behind a condition on `ok`: a warp whose wait ran out makes none."""
+    lines = source.splitlines()
+    at = [i for i, line in enumerate(lines) if arrival in line]
+    assert at, arrival
+    return all("ok" in lines[i - 1] or "ok" in lines[i].split(arrival)[0] for i in at)
+
+
 # ---- prompts: copies, products, two warps that watch the ring, sixteen of the softmax ----
 
 KB = 1024
@@ -49,12 +57,15 @@ def prompt_run(config, n, **schedule):
     slots, buffers = _prompt_config(*config)
     source = _source("attn_prompt.cu")
     empty_arrivals = _number(source, "EMPTY_ARRIVALS", 1)
+    careful = all(_only_if_ok(source, a) for a in ("mbar_arrive(&hd->p_full[buf])", "mbar_arrive(&hd->p_full[(2", "mbar_arrive_n(&hd->p_full["))
+    drained, needed_only = "hd->drain" in source, "again(" in source
     run = Run(**schedule)
     ahead, steps = (buffers - 1, 2 * n) if two else (buffers, n)
     full, empty = [Bar(1) for _ in range(slots)], [Bar(empty_arrivals) for _ in range(slots)]
     s_full, p_full = [Bar(1) for _ in range(buffers)], [Bar(_number(source, "P_ARRIVALS")) for _ in range(buffers)]
     o_full, q_full = [Bar(1), Bar(1)], Bar(16)
     softmax, chains, end = Meeting(16), [Meeting(8), Meeting(8)], Meeting(20)
+    drain = Bar(1)
     content, scores_of, product = [None] * slots, [None] * buffers, [None]
     untaken, left = [0], [0] * buffers  # warps that have yet to take the product; warps that have left their weights over the scores
 
@@ -62,7 +73,7 @@ def prompt_run(config, n, **schedule):
         content[slot] = tile
 
     def copies():
-        kj = vj = 0
+        kj = vj = issued = 0
         for at in range(2 * n):
             is_v = not (kj < n and kj < ahead + vj)
             tile = ("v", vj) if is_v else ("k", kj)
@@ -74,6 +85,10 @@ def prompt_run(config, n, **schedule):
             content[s] = None
             full[s].arrive(tx=1)
             run.copies.append((full[s], lambda s=s, tile=tile: land(s, tile)))
+            issued += 1
+        if drained:
+            for at in range(max(0, issued - slots), issued):
+                yield full[at % slots], (at // slots) & 1, True
         yield end, end.join()
 
     def use(slot, tile, t, buf, is_scores):
@@ -88,10 +103,11 @@ def prompt_run(config, n, **schedule):
     def products():
         def issue(t, is_scores):
             j, buf = (t >> 1 if two else t), t % buffers
-            s = (k_at(j, ahead) if is_scores else v_at(j, n, ahead)) % slots
+            at = k_at(j, ahead) if is_scores else v_at(j, n, ahead)
+            s = at % slots
             run.products.append(lambda: use(s, ("k" if is_scores else "v", j), t, buf, is_scores))
             run.products.append(lambda: (s_full[buf] if is_scores else o_full[t & 1]).arrive())
-            if not two or t & 1:
+            if (not two or t & 1) and not (needed_only and at + slots >= 2 * n):
                 run.products.append(lambda: empty[s].arrive())
 
         ok = yield q_full, 0
@@ -111,6 +127,9 @@ def prompt_run(config, n, **schedule):
             issue(t, False)
             if t + buffers < steps:
                 issue(t + buffers, True)
+        if drained:
+            run.products.append(drain.arrive)
+            yield drain, 0, True
         yield end, end.join()
 
     def watcher(first):
@@ -129,9 +148,10 @@ def prompt_run(config, n, **schedule):
                     run.check(content[at % slots] == ("v", j), "a watcher cleans", content[at % slots], "for", j)
             if t >= buffers and ok:
                 ok = yield p_full[t % buffers], (t // buffers - 1) & 1
+            if ok or not careful:
+                p_full[t % buffers].arrive(1 + 8 if t == 0 and first else 1)
             if not ok:
                 break
-            p_full[t % buffers].arrive(1 + 8 if t == 0 and first else 1)
         yield end, end.join()
 
     def weights(chain):
@@ -146,12 +166,13 @@ def prompt_run(config, n, **schedule):
             yield chains[chain], chains[chain].join()
             left[t % buffers] += 1
             yield None
-            p_full[t % buffers].arrive()
+            if ok or not careful:
+                p_full[t % buffers].arrive()
             ok = ok and (yield o_full[chain], use_ & 1)
             run.check(product[0] == t, "product", product[0], "for", t)
             untaken[0] -= 1
             yield None
-            if t + 1 < steps:
+            if t + 1 < steps and (ok or not careful):
                 p_full[(t + 1) % buffers].arrive()
             use_ += 1
         yield softmax, softmax.join()
@@ -177,3 +198,12 @@ def test_prompt_ring_holds_whichever_warp_is_late(config):
         for warp in WARPS[:6]:
             for turns in range(0, 14):
                 prompt_run(config, n, seed=turns, held=(warp, turns))
+
+
+@pytest.mark.parametrize("config", CONFIGS)
+def test_prompt_block_ends_clean_when_a_wait_runs_out(config):
+    """Whatever wait runs out: no barrier gets an arrival that its phase does not expect beside bytes in flight, and the block does not end
+    before its copies and products."""
+    for n in (1, 3, 6):
+        for seed in range(60):
+            prompt_run(config, n, seed=seed, give_up=0.002 * (1 + seed % 5), late=((), ("watcher 2",), ("copies",), ("products",))[seed % 4])
