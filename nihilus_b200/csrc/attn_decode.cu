@@ -14,6 +14,9 @@
 // running sums are f32 FMAs, because the tensor cores truncate.  (bf16 parts hold 8 bits each: a third one takes a product of its
 // own, in rows 0-7.)
 //
+// Every wait is bounded; one that runs out is recorded for the host.  A warp whose wait ran out goes on without waiting, so that what
+// other CTAs count on is counted, but arrives nowhere in its own any more: a slot is never filled while a copy into it is in flight.
+//
 // The warps work ahead of one another over the (sequence, kv head) pieces of a stretch: the producer fetches the next piece's
 // queries and tiles, the compute warps leave a piece's eight partial results in one of two buffers and go on, and two finishing
 // warps join them with what other CTAs and the shared prefix contribute.
@@ -281,6 +284,7 @@ namespace nhb {
 				uint32_t ph		   = 1;
 				bool ok			   = true;
 				int number = 0;// of the piece
+				int issued = 0, q_issued = 0;// copies of tiles and of queries (lane 0)
 				long long x = x0;
 				piece_t at, then;
 				bool more = next_piece(cum, n, units, x, x1, at);
@@ -308,10 +312,10 @@ namespace nhb {
 						const int head0 = (at.unit - kvh * p.blocks) * ROWS, b = number & 1;
 						const int bytes = min(ROWS, p.a.group - head0) * D * 4;
 						if (!mbar_wait(&hd->q_empty[b], ((number >> 1) & 1) ^ 1)) {
-							atomicExch(p.c.status, DEV_TIMEOUT_EMPTY);
 							ok = false;
 						} else {
 							mbar_expect_tx(&hd->q_full[b], bytes);
+							++q_issued;
 							bulk_g2s_plain(smem_u32(qs + b * ROWS * D), p.a.q + static_cast<long long>(at.i) * p.a.ldq + static_cast<long long>(kvh * p.a.group + head0) * D, bytes, &hd->q_full[b]);
 						}
 					}
@@ -329,10 +333,10 @@ namespace nhb {
 						}
 						if (lane == 0) {
 							if (!mbar_wait(&hd->empty[s], ph)) {
-								atomicExch(p.c.status, DEV_TIMEOUT_EMPTY);
 								ok = false;
 							} else {
 								mbar_expect_tx(&hd->full[s], boxes * 2 * PANELS * box_rows * 128);
+								++issued;
 							}
 						}
 						ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -350,6 +354,15 @@ namespace nhb {
 						}
 					}
 					at = then;
+				}
+				// the last copy into each buffer has landed before the block ends
+				if (lane == 0) {
+					for (int i = max(0, issued - NST); i < issued; ++i)
+						ok = mbar_wait(&hd->full[i % NST], (i / NST) & 1) && ok;
+					for (int i = max(0, q_issued - 2); i < q_issued; ++i)
+						ok = mbar_wait(&hd->q_full[i & 1], (i >> 1) & 1) && ok;
+					if (!ok)
+						atomicExch(p.c.status, DEV_TIMEOUT_EMPTY);
 				}
 				return;
 			}
@@ -403,8 +416,7 @@ namespace nhb {
 						add_prefix(r, at.i, kvh, head0 + h);// while the keys are still being read
 					if (ok && !mbar_wait(&hd->part_full[b], (number >> 1) & 1)) {
 						ok = false;
-						if (lane == 0)
-							atomicExch(p.c.status, DEV_TIMEOUT_DRAIN);
+						atomicExch(p.c.status, DEV_TIMEOUT_DRAIN);
 					}
 					const part_ml& pm = ms[b];
 					float top		  = -INFINITY;
@@ -428,7 +440,7 @@ namespace nhb {
 						}
 					}
 					__syncwarp();
-					if (lane == 0)
+					if (lane == 0 && ok)
 						mbar_arrive(&hd->part_empty[b]);
 					if (c0 == c1) {
 						if (mine) {
@@ -500,8 +512,7 @@ namespace nhb {
 					const int b = number & 1;
 					if (ok && !mbar_wait(&hd->q_full[b], (number >> 1) & 1)) {
 						ok = false;
-						if (lane == 0)
-							atomicExch(p.c.status, DEV_TIMEOUT_FULL);
+						atomicExch(p.c.status, DEV_TIMEOUT_FULL);
 					}
 					const float* src = qs + (b * ROWS + g) * D + 2 * t4;
 					float amax		 = 0.f;
@@ -530,7 +541,7 @@ namespace nhb {
 					if (g >= heads)
 						factor = p.a.scale2;
 					__syncwarp();
-					if (lane == 0)
+					if (lane == 0 && ok)
 						mbar_arrive(&hd->q_empty[b]);
 				}
 				float m = -INFINITY, l = 0.f;
@@ -544,8 +555,7 @@ namespace nhb {
 					const int s = count % NST;
 					if (ok && !mbar_wait(&hd->full[s], (count / NST) & 1)) {
 						ok = false;
-						if (lane == 0)
-							atomicExch(p.c.status, DEV_TIMEOUT_FULL);
+						atomicExch(p.c.status, DEV_TIMEOUT_FULL);
 					}
 					const uint32_t st = smem_u32(base) + s * STAGE;
 					const int left	  = keys - t * KT - wk;// valid keys from this warp's first on
@@ -620,7 +630,7 @@ namespace nhb {
 					if (left < 16)
 						fence_proxy_async();// the zeroed rows, before the next tile is copied over them
 					__syncwarp();
-					if (lane == 0)
+					if (lane == 0 && ok)
 						mbar_arrive(&hd->empty[s]);
 				}
 				// ---- this warp's part of the piece ----
@@ -629,8 +639,7 @@ namespace nhb {
 				const int b = number & 1;
 				if (ok && !mbar_wait(&hd->part_empty[b], ((number >> 1) & 1) ^ 1)) {
 					ok = false;
-					if (lane == 0)
-						atomicExch(p.c.status, DEV_TIMEOUT_EMPTY);
+					atomicExch(p.c.status, DEV_TIMEOUT_EMPTY);
 				}
 				if (t4 == 0) {
 					ms[b].m[warp][g] = m;
@@ -641,7 +650,7 @@ namespace nhb {
 					for (int j = 0; j < D / 8; ++j)
 						*reinterpret_cast<float2*>(mo + ((b * WARPS + warp) * ROWS + g) * D + 8 * j + 2 * t4) = make_float2(o[j][0], o[j][1]);
 				__syncwarp();
-				if (lane == 0)
+				if (lane == 0 && ok)
 					mbar_arrive(&hd->part_full[b]);
 			}
 		}

@@ -207,3 +207,106 @@ def test_prompt_block_ends_clean_when_a_wait_runs_out(config):
     for n in (1, 3, 6):
         for seed in range(60):
             prompt_run(config, n, seed=seed, give_up=0.002 * (1 + seed % 5), late=((), ("watcher 2",), ("copies",), ("products",))[seed % 4])
+
+
+# ---- decode: copies, eight compute warps in two teams, two finishing warps ----
+
+
+def decode_run(slots, pieces, **schedule):
+    """A CTA over pieces of so many tiles each."""
+    source = _source("attn_decode.cu")
+    careful = all(_only_if_ok(source, f"mbar_arrive(&hd->{b}[") for b in ("q_empty", "empty", "part_full", "part_empty"))
+    drained = "issued" in source
+    run = Run(**schedule)
+    full, empty = [Bar(1) for _ in range(slots)], [Bar(4) for _ in range(slots)]
+    q_full, q_empty = [Bar(1), Bar(1)], [Bar(8), Bar(8)]
+    part_full, part_empty = [Bar(8), Bar(8)], [Bar(2), Bar(2)]
+    content, queries, parts = [None] * slots, [None, None], [[None] * 8, [None] * 8]
+
+    def copy(bar, where, i, what):
+        where[i] = None
+        bar.arrive(tx=1)
+        run.copies.append((bar, lambda: where.__setitem__(i, what)))
+
+    def copies():
+        issued = q_issued = 0
+        ok = True
+        for number, tiles in enumerate(pieces):
+            b = number & 1
+            ok = yield q_empty[b], ((number >> 1) & 1) ^ 1
+            if not ok:
+                break
+            copy(q_full[b], queries, b, number)
+            q_issued += 1
+            for _ in range(tiles):
+                s = issued % slots
+                ok = yield empty[s], ((issued // slots) & 1) ^ 1
+                if not ok:
+                    break
+                copy(full[s], content, s, issued)
+                issued += 1
+            if not ok:
+                break
+        if drained:
+            for at in range(max(0, issued - slots), issued):
+                yield full[at % slots], (at // slots) & 1, True
+            for at in range(max(0, q_issued - 2), q_issued):
+                yield q_full[at & 1], (at >> 1) & 1, True
+
+    def compute(warp):
+        ok, count = True, 0
+        for number, tiles in enumerate(pieces):
+            b = number & 1
+            ok = ok and (yield q_full[b], (number >> 1) & 1)
+            run.check(queries[b] == number, "queries", queries[b], "for", number)
+            if ok or not careful:
+                q_empty[b].arrive()
+            for _ in range(tiles):
+                if count & 1 == warp >> 2:
+                    s = count % slots
+                    ok = ok and (yield full[s], (count // slots) & 1)
+                    run.check(content[s] == count, "a tile", content[s], "for", count)
+                    yield None
+                    run.check(content[s] == count, "a tile in use is overwritten")
+                    if ok or not careful:
+                        empty[s].arrive()
+                count += 1
+            ok = ok and (yield part_empty[b], ((number >> 1) & 1) ^ 1)
+            parts[b][warp] = number
+            if ok or not careful:
+                part_full[b].arrive()
+
+    def finish():
+        ok = True
+        for number in range(len(pieces)):
+            b = number & 1
+            ok = ok and (yield part_full[b], (number >> 1) & 1)
+            run.check(parts[b] == [number] * 8, "parts", parts[b], "for", number)
+            yield None
+            run.check(parts[b] == [number] * 8, "parts in use are overwritten")
+            if ok or not careful:
+                part_empty[b].arrive()
+
+    run.warps = {"copies of tiles": copies(), "finish 0": finish(), "finish 1": finish(), **{f"compute {w}": compute(w) for w in range(8)}}
+    run.go()
+
+
+PIECES = [[1], [2, 1], [9], [3, 1, 1, 4, 2], [1] * 9, [12, 5]]
+
+
+@pytest.mark.parametrize("slots", [4, 8])
+def test_decode_ring_holds_whichever_warp_is_late(slots):
+    for pieces in PIECES:
+        for late in [()] + [(w,) for w in ("copies of tiles", "finish 0", "compute 0", "compute 5", "copies")] + [("compute 0", "compute 1", "compute 2", "compute 3")]:
+            for seed in range(4):
+                decode_run(slots, pieces, seed=seed, late=late)
+        for warp in ("copies of tiles", "finish 1", "compute 3", "compute 4"):
+            for turns in range(12):
+                decode_run(slots, pieces, seed=turns, held=(warp, turns))
+
+
+@pytest.mark.parametrize("slots", [4, 8])
+def test_decode_block_ends_clean_when_a_wait_runs_out(slots):
+    for pieces in PIECES:
+        for seed in range(150):
+            decode_run(slots, pieces, seed=seed, give_up=0.005 * (1 + seed % 5), late=((), ("compute 2",), ("copies",), ("finish 0",))[seed % 4])
