@@ -224,7 +224,8 @@ int nhb_last_token_logits(nhb_ctx* ctx, const nhb_weight* w_output, const float*
  * gives the packed token rows of list entry i as cu[i] .. cu[i + 1] - 1; NULL stands for one token each.
  * What the device finds wrong (a sequence or page number out of range, the same sequence twice where the call says so, a length
  * beyond the table) is never followed: nothing is read or written out of bounds and the next nhb_sync returns NHB_ERR_ARG; too few
- * free pages return NHB_ERR_NOMEM there. */
+ * free pages return NHB_ERR_NOMEM there.  Once a reserve has been refused, reserve and append change nothing until nhb_sync has
+ * returned that error: the rows of the step have no place, and would fall on the sequences' older tokens. */
 enum nhb_kv_type { NHB_KV_F16 = 0, NHB_KV_BF16 = 1 };
 typedef struct nhb_kv_cache {
 	void *k, *v; /* device */

@@ -9,7 +9,7 @@
 #include "../../include/nihilus_b200.h"
 
 #define NHB_MAX_BATCH 8
-#define NHB_STATUS_WORDS 8
+#define NHB_STATUS_WORDS 8// the first: what went wrong; KV_REFUSED (kv_cache.h): the K/V cache waits for nhb_sync
 #define NHB_MAX_WORLD 8
 
 namespace nhb {

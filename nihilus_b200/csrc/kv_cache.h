@@ -9,6 +9,10 @@
 
 namespace nhb {
 
+	// Status word that a refused nhb_kv_reserve sets beside the first.  Until nhb_sync has reported it, reserve and append change nothing: the
+	// last tokens of a sequence are then not those that the caller appends, and storing them would overwrite older ones.
+	constexpr int KV_REFUSED = 1;
+
 	// nhb_kv_cache with 32-bit sizes (check_cache has found that they fit)
 	struct kv_view {
 		char* k;// [n_layers][n_pages][kv_heads][page_tokens][head_dim], 2-byte values
@@ -18,7 +22,7 @@ namespace nhb {
 		int32_t* refs;// [n_pages]
 		int n_layers, n_pages, kv_heads, page_tokens, page_shift, head_dim, max_seqs, max_pages;
 		int bf16;
-		int* status;// the context's device status word
+		int* status;// the context's device status words (KV_REFUSED: the second)
 		long long layer_bytes;// of k and of v
 	};
 

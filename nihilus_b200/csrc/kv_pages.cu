@@ -116,6 +116,7 @@ namespace nhb {
 			__shared__ long long wide_scan[32];
 			pdl_launch_dependents();
 			pdl_wait_prior_grids();
+			const int refused  = __ldcg(c.status + KV_REFUSED);// (on its way beside the lookups)
 			const plan_lists l = lists_at(ws, n, c.n_pages);
 			const int tid	   = threadIdx.x;
 			for (int i = tid; i < (c.max_seqs + 31) / 32; i += PLAN_THREADS)
@@ -146,15 +147,19 @@ namespace nhb {
 					l.base[i] = static_cast<int>(total + at);// only read where the total fits
 				total += sum;
 			}
-			if (__syncthreads_or(bad)) {
-				if (tid == 0)
+			if (__syncthreads_or(bad) || refused) {
+				if (tid == 0 && !refused) {
 					report(c.status, DEV_KV_BAD);
+					c.status[KV_REFUSED] = 1;
+				}
 				return;
 			}
 			// (most decode steps open no page at all and skip the search)
 			if (total > c.n_pages || (total > 0 && collect(c.refs, 0, c.n_pages, true, l.dst, static_cast<int>(total), scan) < total)) {
-				if (tid == 0)
+				if (tid == 0) {
 					report(c.status, DEV_KV_NO_PAGES);
+					c.status[KV_REFUSED] = 1;
+				}
 				return;
 			}
 			__syncthreads();// base and dst are written

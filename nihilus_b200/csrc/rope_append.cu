@@ -64,11 +64,12 @@ namespace nhb {
 			pdl_launch_dependents();
 			pdl_wait_prior_grids();
 			const int t = blockIdx.x, tid = threadIdx.x;
+			const int refused = __ldcg(c.status + KV_REFUSED);// (on its way beside the lookups)
 			const int e = entry_of(a.cu, a.n, t, &slot);
 			if (e < 0)
 				return;
 			const int s = a.seqs[e];
-			if (s == -1)
+			if (s == -1 || refused)
 				return;
 			// the position, and where the token's rows of the cache lie; a token the table has no page for is reported and skipped
 			bool sound	   = s >= 0 && s < c.max_seqs;

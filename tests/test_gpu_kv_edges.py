@@ -1,0 +1,54 @@
+"""Calls at the edges of what the K/V cache and its attention allow, on a B200: refused steps, damaged tables, far ranges, long lists, other
+streams.  Tolerances as in test_gpu_kv_cache.py."""
+import math
+import random
+
+import numpy as np
+import pytest
+
+from tests import kv_model
+from tests.test_gpu_kv_cache import _build, _check_rows, _t
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx(capi):
+    c = capi.Context(0)
+    c.use_torch_stream()
+    yield c
+    c.close()
+
+
+def _same(a, b):
+    return bool(((a == b) | ((a != a) & (b != b))).all())
+
+
+# ---- pages ----
+
+
+def test_rows_of_a_refused_step_are_not_stored(capi, ctx):
+    """Too few pages, or a list that is unsound: the append behind it, and the steps behind that, leave cache and rows as they were until
+    the error has been returned; then the step can be made again."""
+    import torch
+
+    cache = _build(capi, "f16", [20, 33, 0], 1, 64, 16, 1, spare=2, max_tokens=200)
+    rope = capi.Rope()
+    x = torch.randn((90, 64), device="cuda")
+    seqs, cu = _t([0, 1]), _t([0, 30, 90])
+    for bad, code in ((lambda: ctx.kv_reserve(cache, seqs, cu), capi.ERR_NOMEM), (lambda: ctx.kv_reserve(cache, _t([0, 0])), capi.ERR_ARG)):
+        before = [t.clone() for t in (cache.k, cache.v, cache.table, cache.lens, cache.refs)]
+        out = torch.full_like(x, 2.0)
+        bad()
+        ctx.rope_kv_append(cache, 0, x, x, x, seqs, cu, rope, q_out=out)
+        ctx.kv_reserve(cache, _t([0]))  # the next step of a loop that does not look
+        ctx.rope_kv_append(cache, 0, x[:1], x[:1], x[:1], _t([0]), None, rope, q_out=out[:1])
+        with pytest.raises(capi.NhbError) as e:
+            ctx.sync()
+        assert e.value.code == code
+        assert all(_same(a, b) for a, b in zip(before, (cache.k, cache.v, cache.table, cache.lens, cache.refs))) and (out == 2.0).all()
+    ctx.kv_reserve(cache, _t([0]))
+    ctx.rope_kv_append(cache, 0, x[:1], x[:1], x[:1], _t([0]), None, None)
+    ctx.sync()
+    assert cache.lens.tolist() == [21, 33, 0]
+    assert torch.equal(cache.v[0, cache.table[0, 1].long(), 0, 4], x[0].half())
