@@ -186,14 +186,14 @@ namespace nhb {
 		// ---- fork: the plan (one CTA), then tables and copies ----
 		__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(kv_view c, const int* __restrict__ parents, const int* __restrict__ children, int n, int deep,
 			void* ws) {
-			extern __shared__ unsigned bits[];
+			extern __shared__ unsigned bits[];// one bit per sequence: children, then parents that have been looked at
 			__shared__ int scan[32];
 			__shared__ long long wide_scan[32];
 			pdl_launch_dependents();
 			pdl_wait_prior_grids();
 			const plan_lists l = lists_at(ws, n, c.n_pages);
 			const int tid	   = threadIdx.x;
-			for (int i = tid; i < (c.max_seqs + 31) / 32; i += PLAN_THREADS)
+			for (int i = tid; i < 2 * ((c.max_seqs + 31) / 32); i += PLAN_THREADS)
 				bits[i] = 0;
 			__syncthreads();
 			bool bad		= false;
@@ -214,9 +214,23 @@ namespace nhb {
 				total += sum;
 			}
 			__syncthreads();// all children are marked
-			for (int i = tid; i < n; i += PLAN_THREADS)
-				if (children[i] != -1 && parents[i] >= 0 && parents[i] < c.max_seqs && ((bits[parents[i] >> 5] >> (parents[i] & 31)) & 1u))
+			// a parent is nobody's child, and its table (looked at once, by a warp) holds pages only
+			const int lane	 = tid & 31;
+			unsigned* looked = bits + (c.max_seqs + 31) / 32;
+			for (int i = tid >> 5; i < n; i += PLAN_THREADS / 32) {
+				const int p = parents[i];
+				if (children[i] == -1 || p < 0 || p >= c.max_seqs)
+					continue;
+				if ((bits[p >> 5] >> (p & 31)) & 1u)
 					bad = true;
+				const int tokens = c.lens[p];
+				if (__shfl_sync(0xffffffffu, lane == 0 ? mark(looked, p) : false, 0) || tokens < 0 || tokens > kv_capacity(c))
+					continue;
+				const int* row = c.table + static_cast<size_t>(p) * c.max_pages;
+				for (int j = lane; j < kv_pages_of(c, tokens); j += 32)
+					if (row[j] < 0 || row[j] >= c.n_pages)
+						bad = true;
+			}
 			if (__syncthreads_or(bad)) {
 				if (tid == 0) {
 					l.head->ok = 0;
@@ -232,7 +246,6 @@ namespace nhb {
 				return;
 			}
 			__syncthreads();
-			const int lane = tid & 31;
 			for (int i = tid >> 5; i < n; i += PLAN_THREADS / 32) {
 				if (children[i] == -1)
 					continue;
@@ -240,15 +253,9 @@ namespace nhb {
 				const int held = kv_pages_of(c, tokens), first = deep ? 0 : tokens >> c.page_shift;
 				const int* row = c.table + static_cast<size_t>(parents[i]) * c.max_pages;
 				for (int j = first + lane; j < held; j += 32) {
-					const int at = l.base[i] + j - first;
-					int page	 = row[j], rows = min(c.page_tokens, tokens - (j << c.page_shift));
-					if (page < 0 || page >= c.n_pages) {
-						report(c.status, DEV_KV_BAD);
-						page = 0;
-						rows = 0;// nothing is copied
-					}
-					l.src[at]		   = page;
-					l.rows[at]		   = rows;
+					const int at	  = l.base[i] + j - first;
+					l.src[at]		  = row[j];
+					l.rows[at]		  = min(c.page_tokens, tokens - (j << c.page_shift));
 					c.refs[l.dst[at]] = 1;
 				}
 			}
@@ -307,10 +314,7 @@ namespace nhb {
 					int page = -1;
 					if (j < shared) {
 						page = from[j];
-						if (page >= 0 && page < c.n_pages)
-							atomicAdd(c.refs + page, 1);
-						else
-							report(c.status, DEV_KV_BAD);
+						atomicAdd(c.refs + page, 1);
 					} else if (j < held) {
 						page = __ldcg(l.dst + __ldcg(l.base + i) + j - shared);
 					}
@@ -630,7 +634,7 @@ int nhb_kv_fork(nhb_ctx* ctx, const nhb_kv_cache* cache, const int32_t* parents_
 	if (rc != NHB_OK)
 		return rc;
 	const int dp  = deep != 0;
-	cudaError_t e = kv_launch(ctx, kv_fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), bitmap_bytes(c), c, parents_dev, children_dev, static_cast<int>(n), dp, ws);
+	cudaError_t e = kv_launch(ctx, kv_fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), 2 * bitmap_bytes(c), c, parents_dev, children_dev, static_cast<int>(n), dp, ws);
 	if (e == cudaSuccess)
 		e = kv_launch(ctx, kv_fork_apply_kernel, dim3(copy_grid(ctx, static_cast<double>(n) * (dp ? c.max_pages : 1) * c.n_layers * 2 * c.kv_heads, n)), dim3(256), 0, c, parents_dev, children_dev, static_cast<int>(n), dp, ws);
 	return e == cudaSuccess ? NHB_OK : fail_cuda(ctx, e, "kv_fork launch");

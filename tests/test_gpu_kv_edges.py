@@ -52,3 +52,26 @@ def test_rows_of_a_refused_step_are_not_stored(capi, ctx):
     ctx.sync()
     assert cache.lens.tolist() == [21, 33, 0]
     assert torch.equal(cache.v[0, cache.table[0, 1].long(), 0, 4], x[0].half())
+
+
+def test_a_fork_of_a_damaged_table_changes_nothing(capi, ctx):
+    """A page number that is none, in a page to be shared or in the one to be copied, of one parent among several: all or nothing."""
+    import torch
+
+    cache = _build(capi, "bf16", [40, 0, 33, 0, 0, 7], 2, 64, 16, 1, spare=6, max_tokens=64)
+    for column, number in ((0, 99), (1, -5), (2, 1 << 30), (0, -1)):
+        for deep in (False, True):
+            good = cache.table[0, column].item()
+            cache.table[0, column] = number
+            before = [t.clone() for t in (cache.table, cache.lens, cache.refs, cache.k, cache.v)]
+            ctx.kv_fork(cache, _t([2, 0, 0]), _t([1, 3, 4]), deep=deep)
+            with pytest.raises(capi.NhbError) as e:
+                ctx.sync()
+            assert e.value.code == capi.ERR_ARG
+            assert all(_same(a, b) for a, b in zip(before, (cache.table, cache.lens, cache.refs, cache.k, cache.v))), (column, number, deep)
+            cache.table[0, column] = good
+    cache.table[0, 3] = 99  # behind the last page: no part of the sequence
+    ctx.kv_fork(cache, _t([0, -1, 2, 0]), _t([3, -1, 1, 4]))
+    ctx.sync()
+    assert cache.lens.tolist() == [40, 33, 33, 40, 40, 7] and cache.table[4, :2].tolist() == cache.table[0, :2].tolist() and cache.table[4, 3] == -1
+    assert cache.refs[cache.table[0, 0].long()] == 3
