@@ -82,8 +82,9 @@ namespace nhb {
 		}
 	}
 
-	// A row of queries is scaled by a power of two that brings its largest element to [2^12, 2^13) before it is split: both 16-bit
+	// A row of queries is scaled by a power of two that brings its largest element to [2^12, 2^13) before it is split for f16: both 16-bit
 	// parts are then normal numbers for all elements that matter, whatever the row's size.  Returns the factor; *back undoes it.
+	// bf16 has f32's range: its rows are split as they are, so that their products with keys of any size stay in range where f32's do.
 	__device__ __forceinline__ float row_scaling(float amax, float* back) {
 		int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127 - 12;
 		if (amax == 0.f || e > 115)// zero, or infinite / NaN / next to the largest f32

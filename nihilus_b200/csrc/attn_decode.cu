@@ -515,17 +515,19 @@ namespace nhb {
 						atomicExch(p.c.status, DEV_TIMEOUT_FULL);
 					}
 					const float* src = qs + (b * ROWS + g) * D + 2 * t4;
-					float amax		 = 0.f;
+					float f = 1.f, back = 1.f;
+					if constexpr (!BF16) {
+						float amax = 0.f;
 #pragma unroll
-					for (int j = 0; j < D / 8; ++j) {
-						const float2 v = *reinterpret_cast<const float2*>(src + 8 * j);
-						amax		   = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+						for (int j = 0; j < D / 8; ++j) {
+							const float2 v = *reinterpret_cast<const float2*>(src + 8 * j);
+							amax		   = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+						}
+						amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+						amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+						f	 = row_scaling(amax, &back);
 					}
-					amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-					amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-					float back;
-					const float f = row_scaling(amax, &back);
-					factor		  = back * p.a.scale2;
+					factor = back * p.a.scale2;
 #pragma unroll
 					for (int j = 0; j < D / 8; ++j) {
 						float2 v = *reinterpret_cast<const float2*>(src + 8 * j);

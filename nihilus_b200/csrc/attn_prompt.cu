@@ -3,7 +3,7 @@
 //
 //   x_j = scale log2(e) q . k_j,   m' = max(m, x),   l' = l 2^(m - m') + sum 2^(x_j - m'),   o' = o 2^(m - m') + sum 2^(x_j - m') v_j
 //
-// f32 accuracy from 16-bit products: a query row is scaled by a power of two and enters as PARTS 16-bit parts (f16: two, 2^-22;
+// f32 accuracy from 16-bit products: a query row (f16: scaled by a power of two) enters as PARTS 16-bit parts (f16: two, 2^-22;
 // bf16: three, 2^-24), the weights likewise, k and v are 16-bit to begin with.  That is PARTS products where one would do for 16-bit
 // rows, and it is what bounds the kernel: 4 head_dim PARTS flops per (row, key).  The tensor cores add into their f32 accumulators by
 // truncation, so one accumulator never holds more than a tile of KT keys; the running sums are f32 FMAs in registers.
@@ -628,7 +628,7 @@ namespace nhb {
 				// two threads per row: one for each half of a tile's columns and of head_dim
 				const int w16 = warp - 4, chain = w16 >> 3, half = (w16 >> 2) & 1;
 				const int lrow = (w16 & 3) * 32 + lane;// row of the tile = lane of tensor memory
-				// ---- queries: scale a row by a power of two, split it, store the parts swizzled; D / 4 lanes per row ----
+				// ---- queries: split a row (f16: scaled by a power of two), store the parts swizzled; D / 4 lanes per row ----
 				{
 					constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
 					const int n_rows = two ? 2 * TILE : TILE;
@@ -647,12 +647,14 @@ namespace nhb {
 						}
 #pragma unroll
 						for (int i = 0; i < BATCH; ++i) {
-							float amax = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+							float f = 1.f, back = 1.f;
+							if constexpr (!BF16) {
+								float amax = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
 #pragma unroll
-							for (int o = LANES / 2; o > 0; o >>= 1)
-								amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-							float back;
-							const float f = row_scaling(amax, &back);
+								for (int o = LANES / 2; o > 0; o >>= 1)
+									amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+								f = row_scaling(amax, &back);
+							}
 							if (rr[i] < n_rows) {
 								uint32_t a[PARTS], b[PARTS];
 								split_parts<BF16>(v[i].x * f, v[i].y * f, a);

@@ -75,3 +75,26 @@ def test_a_fork_of_a_damaged_table_changes_nothing(capi, ctx):
     ctx.sync()
     assert cache.lens.tolist() == [40, 33, 33, 40, 40, 7] and cache.table[4, :2].tolist() == cache.table[0, :2].tolist() and cache.table[4, 3] == -1
     assert cache.refs[cache.table[0, 0].long()] == 3
+
+
+# ---- ranges ----
+
+
+def _both_attentions(capi, ctx, cache, q, scale, heads, d, kind, n):
+    """The prompt call over all rows and the decode call of the last, against the formula with the usual tolerances."""
+    out = ctx.attn_prompt(cache, 0, q, _t([0]), _t([0, n]), scale)
+    last = ctx.attn_decode(cache, 0, q[n - 1 :], _t([0]), scale)
+    ctx.sync()
+    _check_rows(cache, q.reshape(n, heads, d), out.reshape(n, heads, d), [0], [0, n], scale, kind, what="prompt")
+    _check_rows(cache, q[n - 1 :].reshape(1, heads, d), last.reshape(1, heads, d), [0], [0, 1], scale, kind, what="decode")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size, q_size, scale", [(1e35, 1.0, 3e-37), (5e37, 1e-3, 5e-37), (1e-30, 1e3, 3e25), (1e-36, 1e9, 3e25), (1e-36, 1e-2, 3e36)])
+def test_bf16_keys_of_any_size(capi, ctx, d, size, q_size, scale):
+    """Scores of a few units from keys and queries far from 1: what f32 holds is held."""
+    n, heads = 300, 4
+    cache = _build(capi, "bf16", [n], 2, d, 32, 9)
+    cache.k.mul_(size)
+    q = (cache.k.new_empty((n, heads * d)).float().normal_()) * q_size
+    _both_attentions(capi, ctx, cache, q, scale, heads, d, "bf16", n)
