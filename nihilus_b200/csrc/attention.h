@@ -82,6 +82,10 @@ namespace nhb {
 		}
 	}
 
+	// The largest weight of a tile is 2 to this.  f16: 2^14, so that small weights keep all their parts normal numbers; bf16, with f32's range, 1, so
+	// that sums of weights times values stay in range where f32's do.  (Outputs are divided by the sum of the weights.)
+	template<bool BF16> constexpr float WEIGHT_BITS = BF16 ? 0.f : 14.f;
+
 	// A row of queries is scaled by a power of two that brings its largest element to [2^12, 2^13) before it is split for f16: both 16-bit
 	// parts are then normal numbers for all elements that matter, whatever the row's size.  Returns the factor; *back undoes it.
 	// bf16 has f32's range: its rows are split as they are, so that their products with keys of any size stay in range where f32's do.

@@ -601,11 +601,10 @@ namespace nhb {
 					const float mm	 = top == -INFINITY ? 0.f : top;
 					const float keep = ex2(m - mm);
 					m				 = top;
-					// weights up to 2^14: small ones keep both parts normal in f16
 					float w[4];
 #pragma unroll
 					for (int j = 0; j < 4; ++j)
-						w[j] = ex2(x4[j] - mm + 14.f);
+						w[j] = ex2(x4[j] - mm + WEIGHT_BITS<BF16>);
 					l = fmaf(l, keep, (w[0] + w[1]) + (w[2] + w[3]));
 					uint32_t p0[3], p1[3];
 					split_row<BF16>(w[0], w[1], p0);

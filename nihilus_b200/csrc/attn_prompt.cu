@@ -34,7 +34,6 @@ namespace nhb {
 
 		constexpr int PT	   = 640;// threads
 		constexpr int TILE	   = 128;// rows of a tile = tensor-memory lanes
-		constexpr float W_BITS = 14.f;// weights reach 2^14: small ones keep all their parts normal in f16
 
 		constexpr int parts_of(bool bf16) {
 			return bf16 ? 3 : 2;
@@ -177,7 +176,7 @@ namespace nhb {
 			}
 		}
 
-		// The same for weights (positive, at most 2^14), by cutting bits off instead of rounding: a cut float converts exactly, so nothing
+		// The same for weights (positive, at most 2^WEIGHT_BITS), by cutting bits off instead of rounding: a cut float converts exactly, so nothing
 		// has to be converted back to find what is left.  bf16: 8 + 8 + 8 bits are the whole float; f16: 11 + 11 bits, off by at most
 		// 2^-21 (below 2^-14, where f16 becomes subnormal, by at most 2^-25, i.e. 2^-39 of the largest weight).
 		template<bool BF16> __device__ __forceinline__ void cut_parts(float a, float b, uint32_t (&p)[parts_of(BF16)]) {
@@ -725,7 +724,7 @@ namespace nhb {
 					const float mm	 = top == -INFINITY ? 0.f : top;
 					const float keep = ex2(m - mm);
 					m				 = top;
-					const float sum	 = cut ? tile_weights<COLS, BF16, true>(ts, t3, left, factor, W_BITS - mm) : tile_weights<COLS, BF16, false>(ts, t3, left, factor, W_BITS - mm);
+					const float sum	 = cut ? tile_weights<COLS, BF16, true>(ts, t3, left, factor, WEIGHT_BITS<BF16> - mm) : tile_weights<COLS, BF16, false>(ts, t3, left, factor, WEIGHT_BITS<BF16> - mm);
 					tmem_st_wait();
 					tc_fence_before();
 					__syncwarp();

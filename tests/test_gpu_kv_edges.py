@@ -98,3 +98,19 @@ def test_bf16_keys_of_any_size(capi, ctx, d, size, q_size, scale):
     cache.k.mul_(size)
     q = (cache.k.new_empty((n, heads * d)).float().normal_()) * q_size
     _both_attentions(capi, ctx, cache, q, scale, heads, d, "bf16", n)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e35, 1e-36])
+def test_bf16_values_of_any_size(capi, ctx, d, size):
+    """Sums of 300 weights times values that f32 holds, also behind a shared prefix."""
+    n, heads = 300, 4
+    cache = _build(capi, "bf16", [n, n], 2, d, 32, 9)
+    cache.v.mul_(size)
+    q = cache.k.new_empty((n, heads * d)).float().normal_()
+    scale = 1.0 / math.sqrt(d)
+    _both_attentions(capi, ctx, cache, q, scale, heads, d, "bf16", n)
+    cache.table[1, :8] = cache.table[0, :8]
+    out = ctx.attn_decode(cache, 0, q[:2], _t([1, 0]), scale, shared=256)
+    ctx.sync()
+    _check_rows(cache, q[:2].reshape(2, heads, d), out.reshape(2, heads, d), [1, 0], [0, 1, 2], scale, "bf16", what="shared")
