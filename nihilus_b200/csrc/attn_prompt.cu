@@ -352,6 +352,11 @@ namespace nhb {
 					}
 					return static_cast<int>((static_cast<long long>(b - a) * group + TILE * TILES - 1) / (TILE * TILES));
 				};
+				// the grid holds the tiles of M rows; entries that name the same rows (cu falls behind a padding entry) can have more
+				const auto check_grid = [&](int total) {
+					if (blockIdx.x == 0 && tid == 0 && total > static_cast<int>(gridDim.x) / p.c.kv_heads)
+						atomicCAS(p.c.status, DEV_OK, DEV_KV_BAD);
+				};
 				kvh				 = blockIdx.x % p.c.kv_heads;
 				const int rank	 = blockIdx.x / p.c.kv_heads;
 				const bool short_list = p.a.n <= PT;// one look at the list does
@@ -367,6 +372,7 @@ namespace nhb {
 					total = hd->total;
 					if (rank >= total)
 						return;
+					check_grid(total);
 				}
 				int before = 0;
 				for (int i0 = 0; i0 < p.a.n; i0 += PT) {
@@ -392,6 +398,7 @@ namespace nhb {
 						total = all;
 						if (rank >= total)
 							return;
+						check_grid(total);
 					}
 					const int want = total - 1 - rank;
 					if (want >= sum + x - t && want < sum + x) {

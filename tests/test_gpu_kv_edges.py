@@ -114,3 +114,24 @@ def test_bf16_values_of_any_size(capi, ctx, d, size):
     out = ctx.attn_decode(cache, 0, q[:2], _t([1, 0]), scale, shared=256)
     ctx.sync()
     _check_rows(cache, q[:2].reshape(2, heads, d), out.reshape(2, heads, d), [1, 0], [0, 1, 2], scale, "bf16", what="shared")
+
+
+# ---- lists ----
+
+
+def test_rows_that_two_entries_claim_are_reported(capi, ctx):
+    """cu falls behind a padding entry, so that two sequences claim the same rows: more tiles than the call has rows for, in a short and in a
+    long list.  Offsets of padding entries alone may be anything."""
+    import torch
+
+    cache = _build(capi, "f16", [2000, 2000], 2, 64, 16, 4)
+    q = torch.randn((2000, 8 * 64), device="cuda")
+    for pad in (20, 700):
+        ctx.attn_prompt(cache, 0, q, _t([0, -1] * pad + [1]), _t([0, 2000] * (pad + 1)), 0.125)
+        with pytest.raises(capi.NhbError) as e:
+            ctx.sync()
+        assert e.value.code == capi.ERR_ARG
+        seqs, cu = [0] + [-1] * pad + [1], [0, 1000] + [5] * (pad - 1) + [1000, 2000]
+        out = ctx.attn_prompt(cache, 0, q, _t(seqs), _t(cu), 0.125)
+        ctx.sync()
+        _check_rows(cache, q.reshape(-1, 8, 64), out.reshape(-1, 8, 64), [0, 1], [0, 1000, 2000], 0.125, "f16")
