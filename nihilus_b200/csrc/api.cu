@@ -862,11 +862,9 @@ int nhb_ctx_set_stream(nhb_ctx* ctx, void* cuda_stream) {
 	if (!ctx)
 		return fail(nullptr, NHB_ERR_ARG, "null context");
 	const cudaStream_t next = cuda_stream ? static_cast<cudaStream_t>(cuda_stream) : ctx->own;
-	if (next != ctx->stream && (ctx->kv_ws_used || ctx->kv_ws_ev)) {
+	if (next != ctx->stream) {
 		device_guard g(ctx->device);
-		int rc = kv_workspace_follow(ctx, next);
-		if (rc != NHB_OK)
-			return rc;
+		kv_workspace_mark(ctx);// while the stream of the last use is sure to exist; the new one waits when it uses the workspace
 	}
 	ctx->stream = next;
 	return NHB_OK;
@@ -939,6 +937,8 @@ static int sync_enqueue(nhb_ctx* ctx) {
 
 static int sync_finish(nhb_ctx* ctx) {
 	NHB_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+	if (ctx->kv_ws_stream == ctx->stream)
+		ctx->kv_ws_busy = ctx->kv_ws_unmarked = false;
 	if (ctx->host_status[0] != DEV_OK) {
 		const int code = ctx->host_status[0];
 		cudaMemsetAsync(ctx->dev_status, 0, NHB_STATUS_WORDS * sizeof(int), ctx->stream);
@@ -1684,9 +1684,12 @@ int nhb_graph_launch(nhb_ctx* ctx, nhb_graph* gr) {
 	if (!ctx || !gr || !gr->exec)
 		return fail(ctx, NHB_ERR_ARG, "nhb_graph_launch: null argument");
 	device_guard g(ctx->device);
+	if (gr->kv_ws) {
+		int rc = kv_workspace_use(ctx);
+		if (rc != NHB_OK)
+			return rc;
+	}
 	NHB_CUDA(ctx, cudaGraphLaunch(gr->exec, ctx->stream));
-	if (gr->kv_ws)
-		ctx->kv_ws_used = true;
 	replayed(ctx->dl, gr->replay);
 	return NHB_OK;
 }

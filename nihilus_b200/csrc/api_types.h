@@ -76,9 +76,11 @@ struct nhb_ctx {
 	void* kv_ws		 = nullptr;
 	size_t kv_ws_cap = 0;
 	std::vector<void*> kv_ws_old;// outgrown, still named by captured graphs
-	bool kv_ws_used		= false;// on the current stream, since it became the current one
-	bool kv_ws_captured = false;// by the capture that is open
-	cudaEvent_t kv_ws_ev = nullptr;
+	bool kv_ws_busy		   = false;// calls that use it may still be running: all of them before what kv_ws_stream does next ...
+	bool kv_ws_unmarked	   = false;// ... and kv_ws_ev has not been recorded behind the last of them
+	cudaStream_t kv_ws_stream = nullptr;// null once kv_ws_ev is there: the next use waits for that
+	cudaEvent_t kv_ws_ev	   = nullptr;
+	bool kv_ws_captured	   = false;// by the capture that is open
 	std::vector<const void*> kv_smem_set;// kernels that have been given their shared memory on this device
 };
 
@@ -146,8 +148,10 @@ namespace nhb {
 	int ensure(nhb_ctx* ctx, void** buf, size_t* cap, size_t need, const char* what);
 	// in front of work that reads rows another rank may still be delivering: a one-warp kernel that waits for the peers
 	int wait_pending(nhb_ctx* ctx);
-	// the context's stream becomes `next`: it waits for what the old one still does in the K/V workspace
-	int kv_workspace_follow(nhb_ctx* ctx, cudaStream_t next);
+	// K/V workspace: an event behind its last use, if one is missing and can be recorded now (the stream of that use is not being captured)
+	void kv_workspace_mark(nhb_ctx* ctx);
+	// the context's stream, which is not being captured, is about to use the workspace: it comes behind all earlier uses
+	int kv_workspace_use(nhb_ctx* ctx);
 	// Decides what a warp-per-row launch waits for in its prologue and records what it reads and delivers.
 	// in / out: the byte ranges it reads (activations, residual) and writes; `delivers`: the rows in `out` are completed on every rank.
 	void plan_peer_wait(nhb_ctx* ctx, nhb::push_ctl& pc, const nhb_span* in, int n_in, const nhb_span* out, int n_out, bool delivers);

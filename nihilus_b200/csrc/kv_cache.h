@@ -42,8 +42,8 @@ namespace nhb {
 	int check_list(nhb_ctx* ctx, const int32_t* seqs, const int32_t* cu, int64_t n, const char* who);
 	bool rows_overlap(const float* a, int64_t lda, int64_t wa, int64_t ma, const float* b, int64_t ldb, int64_t wb, int64_t mb);
 
-	// One workspace per context for the cache's operators.  Calls follow one another on the context's stream; when the stream
-	// changes, nhb_ctx_set_stream lets the new one wait for the old one's last use.  A buffer that was outgrown is kept until
+	// One workspace per context for the cache's operators.  Calls follow one another on the context's stream; when the stream changes, the first
+	// use on the new one waits for the old one's last.  A buffer that was outgrown is kept until
 	// the context ends: a captured graph may still name it.  In front of the bytes handed out lie NHB_KV_COUNTERS arrival counters
 	// (kv_counters), zero between launches.
 	int kv_workspace(nhb_ctx* ctx, size_t bytes, void** out, const char* who);

@@ -539,6 +539,13 @@ namespace nhb {
 	int kv_workspace(nhb_ctx* ctx, size_t bytes, void** out, const char* who) {
 		cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
 		NHB_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+		if (st == cudaStreamCaptureStatusNone) {
+			if (int rc = kv_workspace_use(ctx); rc != NHB_OK)
+				return rc;
+		} else {
+			// (a capture runs nothing now; its replays are ordered by nhb_graph_launch, or by the caller for a capture of the caller's own)
+			ctx->kv_ws_captured = true;
+		}
 		bytes += NHB_KV_COUNTER_BYTES;
 		if (bytes > ctx->kv_ws_cap) {
 			if (ctx->capturing || st != cudaStreamCaptureStatusNone)
@@ -562,28 +569,39 @@ namespace nhb {
 			ctx->kv_ws	   = p;
 			ctx->kv_ws_cap = want;
 		}
-		if (st == cudaStreamCaptureStatusNone)
-			ctx->kv_ws_used = true;
-		else
-			ctx->kv_ws_captured = true;
 		*out = static_cast<char*>(ctx->kv_ws) + NHB_KV_COUNTER_BYTES;
 		return NHB_OK;
 	}
 
-	int kv_workspace_follow(nhb_ctx* ctx, cudaStream_t next) {
-		// a stream that is being captured runs nothing now: there is nothing to wait for on it, and it does not wait (its replays
-		// are ordered by nhb_graph_launch, or by the caller for a capture of the caller's own)
-		cudaStreamCaptureStatus a = cudaStreamCaptureStatusNone, b = cudaStreamCaptureStatusNone;
-		NHB_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &a));
-		NHB_CUDA(ctx, cudaStreamIsCapturing(next, &b));
-		if (ctx->kv_ws_used && a == cudaStreamCaptureStatusNone) {
+	void kv_workspace_mark(nhb_ctx* ctx) {
+		if (!ctx->kv_ws_busy || !ctx->kv_ws_unmarked)
+			return;
+		// (the query fails for the legacy stream while another stream's capture keeps it from being used: the event comes later)
+		cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+		cudaError_t e			   = cudaStreamIsCapturing(ctx->kv_ws_stream, &st);
+		if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) {
 			if (!ctx->kv_ws_ev)
-				NHB_CUDA(ctx, cudaEventCreateWithFlags(&ctx->kv_ws_ev, cudaEventDisableTiming));
-			NHB_CUDA(ctx, cudaEventRecord(ctx->kv_ws_ev, ctx->stream));
-			ctx->kv_ws_used = false;
+				e = cudaEventCreateWithFlags(&ctx->kv_ws_ev, cudaEventDisableTiming);
+			if (e == cudaSuccess)
+				e = cudaEventRecord(ctx->kv_ws_ev, ctx->kv_ws_stream);
+			if (e == cudaSuccess) {
+				ctx->kv_ws_unmarked = false;
+				ctx->kv_ws_stream	= nullptr;// the stream may end, and another one be given its handle: the next use waits, whatever its stream
+			}
 		}
-		if (ctx->kv_ws_ev && b == cudaStreamCaptureStatusNone)
-			NHB_CUDA(ctx, cudaStreamWaitEvent(next, ctx->kv_ws_ev, 0));
+		if (e != cudaSuccess)
+			cudaGetLastError();
+	}
+
+	int kv_workspace_use(nhb_ctx* ctx) {
+		if (ctx->kv_ws_busy && ctx->kv_ws_stream != ctx->stream) {
+			kv_workspace_mark(ctx);
+			if (ctx->kv_ws_unmarked)
+				return fail(ctx, NHB_ERR_UNSUPPORTED, "the K/V workspace was last used on a stream that cannot be waited for now (it is being captured)");
+			NHB_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->kv_ws_ev, 0));
+		}
+		ctx->kv_ws_stream = ctx->stream;
+		ctx->kv_ws_busy = ctx->kv_ws_unmarked = true;
 		return NHB_OK;
 	}
 

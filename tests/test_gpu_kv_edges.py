@@ -135,3 +135,94 @@ def test_rows_that_two_entries_claim_are_reported(capi, ctx):
         out = ctx.attn_prompt(cache, 0, q, _t(seqs), _t(cu), 0.125)
         ctx.sync()
         _check_rows(cache, q.reshape(-1, 8, 64), out.reshape(-1, 8, 64), [0, 1], [0, 1000, 2000], 0.125, "f16")
+
+
+# ---- streams ----
+
+
+def _cudart():
+    """The CUDA runtime that torch has loaded."""
+    import ctypes as C
+
+    import torch  # noqa: F401  (loads it)
+
+    rt = C.CDLL("libcudart.so.12")
+    for name, args in (("cudaStreamCreate", [C.c_void_p]), ("cudaStreamDestroy", [C.c_void_p]), ("cudaStreamBeginCapture", [C.c_void_p, C.c_int]),
+                       ("cudaStreamEndCapture", [C.c_void_p, C.c_void_p]), ("cudaGraphDestroy", [C.c_void_p])):
+        getattr(rt, name).argtypes, getattr(rt, name).restype = args, C.c_int
+    return rt
+
+
+def _stream(rt):
+    import ctypes as C
+
+    s = C.c_void_p()
+    assert rt.cudaStreamCreate(C.byref(s)) == 0
+    return s.value
+
+
+def test_streams_that_end_between_calls(capi):
+    """A stream may end after nhb_sync, or once another one has been named; what still runs on it is waited for, also where the next stream is
+    given its handle."""
+    import torch
+
+    rt = _cudart()
+    cache = _build(capi, "f16", [9000, 2000, 100], 8, 128, 64, 2)
+    q = torch.randn((3, 32 * 128), device="cuda")
+    seqs = _t([0, 1, 2])
+    outs = [torch.zeros_like(q) for _ in range(24)]
+    with capi.Context(0) as ctx:
+        torch.cuda.synchronize()
+        ref = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        ctx.attn_decode(cache, 0, q, seqs, 0.09, out=ref)
+        ctx.sync()
+        for i, out in enumerate(outs):
+            s = _stream(rt)
+            ctx.set_stream(s)
+            for _ in range(3):
+                ctx.attn_decode(cache, 0, q, seqs, 0.09, out=out)
+            if i % 3 == 0:
+                ctx.sync()
+                assert rt.cudaStreamDestroy(s) == 0
+                ctx.set_stream(None)
+            else:
+                ctx.set_stream(None)
+                assert rt.cudaStreamDestroy(s) == 0
+            if i % 2:
+                ctx.attn_decode(cache, 0, q, seqs, 0.09, out=out)
+        ctx.sync()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, ref) for o in outs)
+
+
+def test_a_capture_open_elsewhere_does_not_hold_the_context_on_the_legacy_stream(capi):
+    """From the legacy stream to a blocking stream that is being captured, and back."""
+    import ctypes as C
+
+    import torch
+
+    rt = _cudart()
+    cache = _build(capi, "f16", [900, 20], 2, 64, 16, 2)
+    q = torch.randn((2, 8 * 64), device="cuda")
+    seqs = _t([0, 1])
+    ref, out, last = (torch.zeros_like(q) for _ in range(3))
+    s, graph = _stream(rt), C.c_void_p()
+    with capi.Context(0) as ctx:
+        ctx.set_stream(1)
+        ctx.attn_decode(cache, 0, q, seqs, 0.125, out=ref)
+        assert rt.cudaStreamBeginCapture(s, 1) == 0
+        try:
+            ctx.set_stream(s)
+            ctx.attn_decode(cache, 0, q, seqs, 0.125, out=out)
+        finally:
+            assert rt.cudaStreamEndCapture(s, C.byref(graph)) == 0
+        ctx.attn_decode(cache, 0, q, seqs, 0.125, out=last)
+        ctx.set_stream(None)
+        ctx.attn_decode(cache, 0, q, seqs, 0.125, out=last)
+        ctx.sync()
+        ctx.set_stream(1)
+        ctx.sync()
+        torch.cuda.synchronize()
+        assert torch.equal(ref, last) and (out == 0).all()  # captured, not run
+    assert rt.cudaGraphDestroy(graph) == 0 and rt.cudaStreamDestroy(s) == 0
