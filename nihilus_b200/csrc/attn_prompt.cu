@@ -291,7 +291,7 @@ namespace nhb {
 			if (reinterpret_cast<unsigned char*>(hd + 1) > smem_raw + prompt_smem(D, BF16, TWO)) {
 				pdl_wait_prior_grids();
 				if (tid == 0)
-					atomicExch(p.c.status, DEV_KV_SMEM);
+					atomicCAS(p.c.status, DEV_OK, DEV_KV_SMEM);
 				return;
 			}
 
