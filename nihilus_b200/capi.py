@@ -389,23 +389,29 @@ class Rope:
     """Rotary embedding (nhb_rope): dims None rotates the whole head; factors: f32 [dims / 2] on the GPU or None."""
 
     def __init__(self, base: float = 500000.0, style: str = "pairs", dims: int | None = None, factors=None):
-        import torch
-
-        if style not in ROPE_STYLES:
-            raise NhbError(ERR_ARG, f"unknown rotary style {style!r}")
-        if factors is not None and (factors.dtype != torch.float32 or factors.dim() != 1 or not factors.is_contiguous() or not factors.is_cuda):
-            raise NhbError(ERR_ARG, "factors must be a contiguous f32 tensor on the GPU")
         self.base, self.style, self.dims, self.factors = float(base), style, dims, factors
-        self._refs = {}  # per head_dim
+        self._check()
+        self._refs = {}  # per head_dim: what the struct was made of, and the struct
+
+    def _check(self):
+        f = self.factors
+        if self.style not in ROPE_STYLES:
+            raise NhbError(ERR_ARG, f"unknown rotary style {self.style!r}")
+        if f is not None and (f.dtype is not _torch_types()[1] or f.dim() != 1 or not f.is_contiguous() or not f.is_cuda):
+            raise NhbError(ERR_ARG, "factors must be a contiguous f32 tensor on the GPU")
 
     def ref(self, head_dim: int):
-        """The C struct for heads of this size, by reference."""
-        if head_dim not in self._refs:
+        """The C struct for heads of this size, by reference; it follows what is assigned to the rotation."""
+        f = self.factors
+        key = (self.base, self.style, self.dims, f.data_ptr() if f is not None else None, f.shape if f is not None else None)
+        made = self._refs.get(head_dim)
+        if made is None or made[0] != key:
+            self._check()
             dims = head_dim if self.dims is None else int(self.dims)
-            if self.factors is not None and self.factors.shape[0] < dims // 2:
+            if f is not None and f.shape[0] < dims // 2:
                 raise NhbError(ERR_ARG, "factors holds fewer than dims / 2 values")
-            self._refs[head_dim] = C.byref(RopeStruct(self.base, dims, ROPE_STYLES[self.style], self.factors.data_ptr() if self.factors is not None else None))
-        return self._refs[head_dim]
+            made = self._refs[head_dim] = (key, C.byref(RopeStruct(self.base, dims, ROPE_STYLES[self.style], key[3])))
+        return made[1]
 
 
 def _check_cu(cu, n: int):
