@@ -400,9 +400,11 @@ class Rope:
         if f is not None and (f.dtype is not _torch_types()[1] or f.dim() != 1 or not f.is_contiguous() or not f.is_cuda):
             raise NhbError(ERR_ARG, "factors must be a contiguous f32 tensor on the GPU")
 
-    def ref(self, head_dim: int):
-        """The C struct for heads of this size, by reference; it follows what is assigned to the rotation."""
+    def ref(self, head_dim: int, device: int | None = None):
+        """The C struct for heads of this size, by reference; it follows what is assigned to the rotation.  device: the GPU that reads the factors."""
         f = self.factors
+        if f is not None and device is not None and f.get_device() != device:
+            raise NhbError(ERR_ARG, "factors lie on another GPU than the context")
         key = (self.base, self.style, self.dims, f.data_ptr() if f is not None else None, f.shape if f is not None else None)
         made = self._refs.get(head_dim)
         if made is None or made[0] != key:
@@ -687,7 +689,7 @@ class Context:
         (qp, ldq), (kp, ldk), (vp, ldv) = _rows32(q, M, width, "q", self.device), _rows32(k, M, kw, "k", self.device), _rows32(v, M, kw, "v", self.device)
         op, ldo = _rows32(q_out, M, width, "q_out", self.device)
         _check(lib.nhb_rope_kv_append(self.handle, self._kv(cache), layer, qp, ldq, _heads(width, cache), kp, ldk, vp, ldv, M, _i32(seqs, "seqs", self.device), _i32(cu, "cu", self.device), n,
-                                      rope.ref(cache.head_dim) if rope is not None else None, op, ldo), self.handle)
+                                      rope.ref(cache.head_dim, self.device) if rope is not None else None, op, ldo), self.handle)
         return q_out
 
     def attn_prompt(self, cache: KvCache, layer: int, q, seqs, cu, scale: float, out=None):

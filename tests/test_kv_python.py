@@ -47,3 +47,79 @@ def test_a_rotation_is_what_was_last_assigned_to_it(capi):
     rope.factors, rope.style = None, "spiral"
     with pytest.raises(capi.NhbError):
         rope.ref(128)
+
+
+class Rows:
+    """Looks like f32 rows on GPU 0."""
+
+    def __init__(self, rows, width, ptr, stride=None):
+        import torch
+
+        self.dtype, self.shape, self.ptr, self.strides = torch.float32, (rows, width), ptr, (stride or width, 1)
+
+    def stride(self):
+        return self.strides
+
+    def data_ptr(self):
+        return self.ptr
+
+    def get_device(self):
+        return 0
+
+
+class List:
+    """Looks like an int32 tensor on GPU 0."""
+
+    def __init__(self, *shape, ptr=1 << 20):
+        import torch
+
+        self.dtype, self.shape, self.ptr = torch.int32, shape, ptr
+
+    def is_contiguous(self):
+        return True
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        n = 1
+        for x in self.shape:
+            n *= x
+        return n
+
+    def data_ptr(self):
+        return self.ptr
+
+    def get_device(self):
+        return 0
+
+
+def _context(capi):
+    """A context of GPU 0 without a handle: calls get as far as the library's own check of it, which comes last."""
+    ctx = capi.Context.__new__(capi.Context)
+    ctx.handle, ctx.device = None, 0
+    return ctx
+
+
+def _cache(capi, max_seqs=4):
+    import ctypes as C
+
+    cache = capi.KvCache.__new__(capi.KvCache)
+    p = 1 << 20
+    struct = capi.KvCacheStruct(p, 2 * p, 3 * p, 4 * p, 5 * p, 1, 8, 2, 16, 64, max_seqs, 4, 0)
+    cache.__dict__.update(kv_heads=2, head_dim=64, device=0, struct=struct, ref=C.byref(struct))
+    return cache
+
+
+def _refused(capi, text, call, *args, **kw):
+    with pytest.raises(capi.NhbError) as e:
+        call(*args, **kw)
+    assert e.value.code == capi.ERR_ARG and text in str(e.value), e.value
+
+
+def test_factors_on_another_gpu_are_refused(capi):
+    ctx, cache = _context(capi), _cache(capi)
+    q, k, v, out = (Rows(2, w, (i + 1) << 24) for i, w in enumerate((256, 128, 128, 256)))
+    here, there = capi.Rope(factors=Factors(32, 4096)), capi.Rope(factors=Factors(32, 4096, device=1))
+    _refused(capi, "null context", ctx.rope_kv_append, cache, 0, q, k, v, List(2), rope=here, q_out=out)  # all else is in order
+    _refused(capi, "another GPU", ctx.rope_kv_append, cache, 0, q, k, v, List(2), rope=there, q_out=out)
