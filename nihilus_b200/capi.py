@@ -663,16 +663,17 @@ class Context:
 
     def kv_reserve(self, cache: KvCache, seqs, cu=None):
         """Room for cu[i + 1] - cu[i] new tokens (cu None: one) of every listed sequence."""
-        _check_cu(cu, seqs.shape[0])
-        _check(lib.nhb_kv_reserve(self.handle, self._kv(cache), _i32(seqs, "seqs", self.device), _i32(cu, "cu", self.device), seqs.shape[0]), self.handle)
+        n = seqs.numel()
+        _check_cu(cu, n)
+        _check(lib.nhb_kv_reserve(self.handle, self._kv(cache), _i32(seqs, "seqs", self.device), _i32(cu, "cu", self.device), n), self.handle)
 
     def kv_fork(self, cache: KvCache, parents, children, deep: bool = False):
         if parents.shape != children.shape:
             raise NhbError(ERR_ARG, "as many children as parents")
-        _check(lib.nhb_kv_fork(self.handle, self._kv(cache), _i32(parents, "parents", self.device), _i32(children, "children", self.device), children.shape[0], int(deep)), self.handle)
+        _check(lib.nhb_kv_fork(self.handle, self._kv(cache), _i32(parents, "parents", self.device), _i32(children, "children", self.device), children.numel(), int(deep)), self.handle)
 
     def kv_free(self, cache: KvCache, seqs):
-        _check(lib.nhb_kv_free(self.handle, self._kv(cache), _i32(seqs, "seqs", self.device), seqs.shape[0]), self.handle)
+        _check(lib.nhb_kv_free(self.handle, self._kv(cache), _i32(seqs, "seqs", self.device), seqs.numel()), self.handle)
 
     def kv_compact(self, cache: KvCache, live=None):
         """live: int32 [1] or None; receives the number of pages in use."""
@@ -681,7 +682,7 @@ class Context:
     def rope_kv_append(self, cache: KvCache, layer: int, q, k, v, seqs, cu=None, rope: Rope | None = None, q_out=None):
         """Rotates q into q_out (None: a new tensor; may be q) and stores rotated k and v as the sequences' last tokens."""
         M, width = q.shape
-        n = seqs.shape[0]
+        n = seqs.numel()
         if q_out is None:
             q_out = q.new_zeros((M, width))
         _check_cu(cu, n)
@@ -695,7 +696,7 @@ class Context:
     def attn_prompt(self, cache: KvCache, layer: int, q, seqs, cu, scale: float, out=None):
         """Causal attention of packed prompt rows (nhb_attn_prompt): q f32 [M][heads * head_dim] -> out."""
         M, width = q.shape
-        n = seqs.shape[0]
+        n = seqs.numel()
         if out is None:
             out = q.new_zeros((M, width))
         _check_cu(cu, n)
@@ -708,7 +709,7 @@ class Context:
         n, width = q.shape
         if out is None:
             out = q.new_zeros((n, width))
-        if seqs.shape[0] != n:
+        if seqs.numel() != n:
             raise NhbError(ERR_ARG, "one row of q per listed sequence")
         (qp, ldq), (op, ldo) = _rows32(q, n, width, "q", self.device), _rows32(out, n, width, "out", self.device)
         _check(lib.nhb_attn_decode(self.handle, self._kv(cache), layer, qp, ldq, _heads(width, cache), _i32(seqs, "seqs", self.device), n, shared, scale, op, ldo), self.handle)

@@ -123,3 +123,34 @@ def test_factors_on_another_gpu_are_refused(capi):
     here, there = capi.Rope(factors=Factors(32, 4096)), capi.Rope(factors=Factors(32, 4096, device=1))
     _refused(capi, "null context", ctx.rope_kv_append, cache, 0, q, k, v, List(2), rope=here, q_out=out)  # all else is in order
     _refused(capi, "another GPU", ctx.rope_kv_append, cache, 0, q, k, v, List(2), rope=there, q_out=out)
+
+
+def test_lists_count_all_their_entries(capi, monkeypatch):
+    """Whatever the shape of a list, as many entries reach the library as it holds."""
+    seen = {}
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: seen.setdefault(name, []).append(args) or 0
+
+    monkeypatch.setattr(capi, "lib", Library())
+    ctx, cache = _context(capi), _cache(capi)
+    for shape in ((6,), (1, 6), (6, 1), (2, 3)):
+        seen.clear()
+        many = List(*shape)
+        q, k, v, out = (Rows(6, w, (i + 1) << 24) for i, w in enumerate((256, 128, 128, 256)))
+        cu = List(7)
+        ctx.kv_reserve(cache, many)
+        ctx.kv_reserve(cache, many, cu)
+        ctx.kv_free(cache, many)
+        ctx.kv_fork(cache, many, List(*shape))
+        ctx.rope_kv_append(cache, 0, q, k, v, many, q_out=out)
+        ctx.attn_prompt(cache, 0, q, many, cu, 0.1, out=out)
+        ctx.attn_decode(cache, 0, q, many, 0.1, out=out)
+        counts = [a[4] for a in seen["nhb_kv_reserve"]] + [a[3] for a in seen["nhb_kv_free"]] + [a[4] for a in seen["nhb_kv_fork"]]
+        counts += [a[13] for a in seen["nhb_rope_kv_append"]] + [a[9] for a in seen["nhb_attn_prompt"]] + [a[7] for a in seen["nhb_attn_decode"]]
+        assert counts == [6] * 7, (shape, counts)
+        with pytest.raises(capi.NhbError):
+            ctx.kv_reserve(cache, many, List(6))
+        with pytest.raises(capi.NhbError):
+            ctx.attn_decode(cache, 0, Rows(5, 256, 1 << 24), many, 0.1, out=Rows(5, 256, 2 << 24))
