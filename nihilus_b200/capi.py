@@ -677,6 +677,8 @@ class Context:
 
     def kv_compact(self, cache: KvCache, live=None):
         """live: int32 [1] or None; receives the number of pages in use."""
+        if live is not None and live.numel() < 1:
+            raise NhbError(ERR_ARG, "live has no room for a number")
         _check(lib.nhb_kv_compact(self.handle, self._kv(cache), _i32(live, "live", self.device)), self.handle)
 
     def rope_kv_append(self, cache: KvCache, layer: int, q, k, v, seqs, cu=None, rope: Rope | None = None, q_out=None):

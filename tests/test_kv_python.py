@@ -154,3 +154,11 @@ def test_lists_count_all_their_entries(capi, monkeypatch):
             ctx.kv_reserve(cache, many, List(6))
         with pytest.raises(capi.NhbError):
             ctx.attn_decode(cache, 0, Rows(5, 256, 1 << 24), many, 0.1, out=Rows(5, 256, 2 << 24))
+
+
+def test_compact_refuses_a_place_without_room(capi):
+    """An empty slice has an address, and the number would land behind it."""
+    ctx, cache = _context(capi), _cache(capi)
+    _refused(capi, "null context", ctx.kv_compact, cache, List(1))
+    _refused(capi, "null context", ctx.kv_compact, cache, List())
+    _refused(capi, "no room", ctx.kv_compact, cache, List(0))
