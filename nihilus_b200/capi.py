@@ -335,7 +335,7 @@ def _rows32(t, rows: int, width: int, what: str, device: int):
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[0] != rows or shape[1] != width or (rows and width > 1 and stride[1] != 1) or t.dtype is not _torch_types()[1] or t.get_device() != device:
         raise NhbError(ERR_ARG, f"{what} must be {rows} f32 rows of {width} on the context's GPU")
-    return t.data_ptr(), (stride[0] if rows > 1 else max(stride[0], width, 1))
+    return t.data_ptr(), (stride[0] if rows > 1 else max(width, 1))  # (one row's stride says nothing)
 
 
 def _torch_types():

@@ -162,3 +162,19 @@ def test_compact_refuses_a_place_without_room(capi):
     _refused(capi, "null context", ctx.kv_compact, cache, List(1))
     _refused(capi, "null context", ctx.kv_compact, cache, List())
     _refused(capi, "no room", ctx.kv_compact, cache, List(0))
+
+
+def test_the_stride_of_one_row_does_not_matter(capi):
+    """A single row of a wider buffer, whatever the buffer's row length."""
+    ctx, cache = _context(capi), _cache(capi)
+    for stride in (256, 260, 261, 1, 0):
+        q, out = Rows(1, 256, 1 << 24, stride), Rows(1, 256, 2 << 24, stride)
+        k, v = Rows(1, 128, 3 << 24, stride), Rows(1, 128, 4 << 24, stride)
+        _refused(capi, "null context", ctx.attn_decode, cache, 0, q, List(1), 0.1, out=out)
+        _refused(capi, "null context", ctx.attn_prompt, cache, 0, q, List(1), List(2), 0.1, out=out)
+        _refused(capi, "null context", ctx.rope_kv_append, cache, 0, q, k, v, List(1), q_out=q)
+    _refused(capi, "rows", ctx.attn_decode, cache, 0, Rows(2, 256, 1 << 24, 261), List(2), 0.1, out=Rows(2, 256, 2 << 24))
+    # a row of q, k and v side by side: they do not meet, and a row that does is refused
+    q, k, v = Rows(1, 256, 1 << 24, 515), Rows(1, 128, (1 << 24) + 1024, 515), Rows(1, 128, (1 << 24) + 1536, 515)
+    _refused(capi, "null context", ctx.rope_kv_append, cache, 0, q, k, v, List(1), q_out=q)
+    _refused(capi, "overlap", ctx.rope_kv_append, cache, 0, q, k, v, List(1), q_out=Rows(1, 256, (1 << 24) + 512, 515))
