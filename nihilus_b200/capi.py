@@ -353,7 +353,12 @@ _types = None
 
 class KvCache:
     """The paged K/V cache over torch tensors (nhb_kv_cache): k, v [layers][pages][kv_heads][page_tokens][head_dim] f16 or bf16,
-    table [max_seqs][max_pages], lens [max_seqs], refs [pages] int32."""
+    table [max_seqs][max_pages], lens [max_seqs], refs [pages] int32.  It is made for these tensors: others take another KvCache."""
+
+    def __setattr__(self, name, value):
+        if name in ("k", "v", "table", "lens", "refs") and self.__dict__.get(name, value) is not value:
+            raise NhbError(ERR_ARG, f"a KvCache is made for its tensors: {name} cannot be replaced")
+        self.__dict__[name] = value
 
     def __init__(self, k, v, table, lens, refs):
         import torch

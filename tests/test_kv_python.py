@@ -178,3 +178,18 @@ def test_the_stride_of_one_row_does_not_matter(capi):
     q, k, v = Rows(1, 256, 1 << 24, 515), Rows(1, 128, (1 << 24) + 1024, 515), Rows(1, 128, (1 << 24) + 1536, 515)
     _refused(capi, "null context", ctx.rope_kv_append, cache, 0, q, k, v, List(1), q_out=q)
     _refused(capi, "overlap", ctx.rope_kv_append, cache, 0, q, k, v, List(1), q_out=Rows(1, 256, (1 << 24) + 512, 515))
+
+
+def test_the_tensors_of_a_cache_cannot_be_replaced(capi):
+    """The C struct holds their pointers: an assignment would be ignored, and the old memory read after its end."""
+    import torch
+
+    cache = _cache(capi)
+    for name in ("k", "v", "table", "lens", "refs"):
+        t = torch.zeros(3)
+        setattr(cache, name, t)
+        setattr(cache, name, t)  # what `cache.k *= 2` does
+        with pytest.raises(capi.NhbError):
+            setattr(cache, name, t.clone())
+        assert getattr(cache, name) is t
+    cache.note = 1
