@@ -481,8 +481,12 @@ class Context:
     def __exit__(self, *a):
         self.close()
 
+    stream = None  # the handle last set (1: the legacy stream); None: the context's own stream
+    capturing = False  # between graph_begin and graph_end
+
     def set_stream(self, cuda_stream: int | None):
         _check(lib.nhb_ctx_set_stream(self.handle, cuda_stream), self.handle)
+        self.stream = cuda_stream or None
 
     def use_torch_stream(self):
         """Run on torch's current stream, so tensors made by torch and kernels launched here are ordered."""
@@ -666,6 +670,18 @@ class Context:
             raise NhbError(ERR_ARG, "the cache lies on another GPU than the context")
         return cache.ref
 
+    def _zeros(self, like, rows: int, width: int):
+        """A new output of zeros.  torch fills it on its own current stream: on another one the context must not come before the fill (a capture
+        runs nothing now, and is replayed after it)."""
+        import torch
+
+        out = like.new_zeros((rows, width))
+        if out.is_cuda and not self.capturing:
+            at = torch.cuda.current_stream(out.device)
+            if (at.cuda_stream or 1) != self.stream and not torch.cuda.is_current_stream_capturing():
+                at.synchronize()
+        return out
+
     def kv_reserve(self, cache: KvCache, seqs, cu=None):
         """Room for cu[i + 1] - cu[i] new tokens (cu None: one) of every listed sequence."""
         n = seqs.numel()
@@ -691,7 +707,7 @@ class Context:
         M, width = q.shape
         n = seqs.numel()
         if q_out is None:
-            q_out = q.new_zeros((M, width))
+            q_out = self._zeros(q, M, width)
         _check_cu(cu, n)
         kw = cache.kv_heads * cache.head_dim
         (qp, ldq), (kp, ldk), (vp, ldv) = _rows32(q, M, width, "q", self.device), _rows32(k, M, kw, "k", self.device), _rows32(v, M, kw, "v", self.device)
@@ -705,7 +721,7 @@ class Context:
         M, width = q.shape
         n = seqs.numel()
         if out is None:
-            out = q.new_zeros((M, width))
+            out = self._zeros(q, M, width)
         _check_cu(cu, n)
         (qp, ldq), (op, ldo) = _rows32(q, M, width, "q", self.device), _rows32(out, M, width, "out", self.device)
         _check(lib.nhb_attn_prompt(self.handle, self._kv(cache), layer, qp, ldq, _heads(width, cache), M, _i32(seqs, "seqs", self.device), _i32(cu, "cu", self.device), n, scale, op, ldo), self.handle)
@@ -715,7 +731,7 @@ class Context:
         """Attention of one row per listed sequence over all its keys; `shared` leading tokens are common to the batch (nhb_attn_decode)."""
         n, width = q.shape
         if out is None:
-            out = q.new_zeros((n, width))
+            out = self._zeros(q, n, width)
         if seqs.numel() != n:
             raise NhbError(ERR_ARG, "one row of q per listed sequence")
         (qp, ldq), (op, ldo) = _rows32(q, n, width, "q", self.device), _rows32(out, n, width, "out", self.device)
@@ -725,9 +741,11 @@ class Context:
     # ---- graphs ----
     def graph_begin(self):
         _check(lib.nhb_graph_begin(self.handle), self.handle)
+        self.capturing = True
 
     def graph_end(self) -> Graph:
         h = _vp()
+        self.capturing = False
         _check(lib.nhb_graph_end(self.handle, C.byref(h)), self.handle)
         return Graph(self, h.value)
 

@@ -226,3 +226,29 @@ def test_a_capture_open_elsewhere_does_not_hold_the_context_on_the_legacy_stream
         torch.cuda.synchronize()
         assert torch.equal(ref, last) and (out == 0).all()  # captured, not run
     assert rt.cudaGraphDestroy(graph) == 0 and rt.cudaStreamDestroy(s) == 0
+
+
+def test_new_outputs_of_a_context_on_another_stream(capi):
+    """torch fills a new output with zeros on its own stream, here behind a long product; the context's rows must not come first."""
+    import torch
+
+    cache = _build(capi, "f16", [90, 20], 2, 64, 16, 2)
+    q, kv = torch.randn((2, 8 * 64), device="cuda"), torch.randn((2, 128), device="cuda")
+    seqs, cu = _t([0, 1]), _t([0, 1, 2])
+    a = torch.randn((8192, 8192), device="cuda")
+    side = torch.cuda.Stream()
+    for stream in (None, side.cuda_stream):
+        with capi.Context(0) as ctx:
+            ctx.set_stream(stream)
+            calls = [lambda **o: ctx.attn_decode(cache, 0, q, seqs, 0.125, **o), lambda **o: ctx.attn_prompt(cache, 0, q, seqs, cu, 0.125, **o),
+                     lambda **o: ctx.rope_kv_append(cache, 0, q, kv, kv, seqs, **{{"out": "q_out"}[k]: v for k, v in o.items()})]
+            for call in calls:
+                ref = torch.zeros_like(q)
+                torch.cuda.synchronize()
+                call(out=ref)
+                ctx.sync()
+                a @ a  # some 15 ms of torch's stream
+                got = call()
+                ctx.sync()
+                torch.cuda.synchronize()
+                assert torch.equal(got, ref) and (got != 0).any()
