@@ -24,8 +24,10 @@ def _ctx():
 
         _lib["capi"] = capi
         _lib["ctx"] = capi.Context(0)
-        _lib["ctx"].use_torch_stream()
-    return _lib["ctx"]
+    ctx = _lib["ctx"]
+    if ctx.stream != (torch.cuda.current_stream().cuda_stream or 1):
+        ctx.use_torch_stream()
+    return ctx
 
 
 # ---- cases ----
