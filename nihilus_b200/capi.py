@@ -351,6 +351,22 @@ def _torch_types():
 _types = None
 
 
+def _torch_stream(device: int) -> int:
+    """The handle of torch's current stream on a GPU."""
+    global _current_stream
+    if _current_stream is None:
+        import torch
+
+        torch.cuda.init()
+        _current_stream = torch._C._cuda_getCurrentRawStream  # (a Stream object costs 3 us)
+    # torch reports its default stream as handle 0, which nhb_ctx_set_stream reads as "the context's own
+    # stream"; 1 is cudaStreamLegacy, the same default stream named explicitly
+    return _current_stream(device) or 1
+
+
+_current_stream = None
+
+
 class KvCache:
     """The paged K/V cache over torch tensors (nhb_kv_cache): k, v [layers][pages][kv_heads][page_tokens][head_dim] f16 or bf16,
     table [max_seqs][max_pages], lens [max_seqs], refs [pages] int32.  It is made for these tensors: others take another KvCache."""
@@ -489,12 +505,11 @@ class Context:
         self.stream = cuda_stream or None
 
     def use_torch_stream(self):
-        """Run on torch's current stream, so tensors made by torch and kernels launched here are ordered."""
-        import torch
-
-        # torch reports its default stream as handle 0, which nhb_ctx_set_stream reads as "the context's own
-        # stream"; 1 is cudaStreamLegacy, the same default stream named explicitly
-        self.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+        """Run on torch's current stream, so tensors made by torch and kernels launched here are ordered.  Cheap where the context is on it
+        already: a program that changes torch's stream may call it in front of every step."""
+        handle = _torch_stream(self.device)
+        if handle != self.stream:
+            self.set_stream(handle)
 
     def set_option(self, name: str, value: int):
         _check(lib.nhb_ctx_set_option(self.handle, name.encode(), value), self.handle)
@@ -676,10 +691,8 @@ class Context:
         import torch
 
         out = like.new_zeros((rows, width))
-        if out.is_cuda and not self.capturing:
-            at = torch.cuda.current_stream(out.device)
-            if (at.cuda_stream or 1) != self.stream and not torch.cuda.is_current_stream_capturing():
-                at.synchronize()
+        if out.is_cuda and not self.capturing and _torch_stream(self.device) != self.stream and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(out.device).synchronize()
         return out
 
     def kv_reserve(self, cache: KvCache, seqs, cu=None):
