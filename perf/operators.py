@@ -24,10 +24,8 @@ def _ctx():
 
         _lib["capi"] = capi
         _lib["ctx"] = capi.Context(0)
-    ctx = _lib["ctx"]
-    if ctx.stream != (torch.cuda.current_stream().cuda_stream or 1):
-        ctx.use_torch_stream()
-    return ctx
+    _lib["ctx"].use_torch_stream()
+    return _lib["ctx"]
 
 
 # ---- cases ----
