@@ -412,7 +412,10 @@ class Rope:
     def __init__(self, base: float = 500000.0, style: str = "pairs", dims: int | None = None, factors=None):
         self.base, self.style, self.dims, self.factors = float(base), style, dims, factors
         self._check()
-        self._refs = {}  # per head_dim: what the struct was made of, and the struct
+
+    def __setattr__(self, name, value):
+        self.__dict__[name] = value
+        self.__dict__["_refs"] = {}  # structs by head size and GPU, of what is assigned now
 
     def _check(self):
         f = self.factors
@@ -423,18 +426,16 @@ class Rope:
 
     def ref(self, head_dim: int, device: int | None = None):
         """The C struct for heads of this size, by reference; it follows what is assigned to the rotation.  device: the GPU that reads the factors."""
-        f = self.factors
-        if f is not None and device is not None and f.get_device() != device:
-            raise NhbError(ERR_ARG, "factors lie on another GPU than the context")
-        key = (self.base, self.style, self.dims, f.data_ptr() if f is not None else None, f.shape if f is not None else None)
-        made = self._refs.get(head_dim)
-        if made is None or made[0] != key:
+        made = self._refs.get((head_dim, device))
+        if made is None:
             self._check()
-            dims = head_dim if self.dims is None else int(self.dims)
+            f, dims = self.factors, head_dim if self.dims is None else int(self.dims)
+            if f is not None and device is not None and f.get_device() != device:
+                raise NhbError(ERR_ARG, "factors lie on another GPU than the context")
             if f is not None and f.shape[0] < dims // 2:
                 raise NhbError(ERR_ARG, "factors holds fewer than dims / 2 values")
-            made = self._refs[head_dim] = (key, C.byref(RopeStruct(self.base, dims, ROPE_STYLES[self.style], key[3])))
-        return made[1]
+            made = self._refs[(head_dim, device)] = C.byref(RopeStruct(self.base, dims, ROPE_STYLES[self.style], f.data_ptr() if f is not None else None))
+        return made
 
 
 def _check_cu(cu, n: int):
