@@ -354,7 +354,7 @@ namespace nhb {
 				};
 				// the grid holds the tiles of M rows; entries that name the same rows (cu falls behind a padding entry) can have more
 				const auto check_grid = [&](int total) {
-					if (blockIdx.x == 0 && tid == 0 && total > static_cast<int>(gridDim.x) / p.c.kv_heads)
+					if (blockIdx.x == 0 && tid == 0 && static_cast<long long>(total) * p.c.kv_heads > gridDim.x)
 						atomicCAS(p.c.status, DEV_OK, DEV_KV_BAD);
 				};
 				kvh				 = blockIdx.x % p.c.kv_heads;
