@@ -137,6 +137,99 @@ def test_rows_that_two_entries_claim_are_reported(capi, ctx):
         _check_rows(cache, q.reshape(-1, 8, 64), out.reshape(-1, 8, 64), [0, 1], [0, 1000, 2000], 0.125, "f16")
 
 
+@pytest.mark.parametrize("n, two", [(1500, False), (641, True), (1281, False), (640, False)])
+def test_prompts_of_more_entries_than_a_block_has_threads(capi, ctx, n, two):
+    """The list is looked at in rounds of 640 entries: padding, entries without rows, of one row and of several tiles, at the rounds' borders
+    too, and one that is unsound, which is reported while the others are computed."""
+    import torch
+
+    r = random.Random(n)
+    heads, kv_heads, d, page = (16, 2, 64, 16) if two else (4, 2, 64, 16)
+    new = [r.choice((0, 1, 1, 2, 5)) for _ in range(n)]
+    for i in (0, 1, 638, 639, 640, 1279, 1280, n - 1):
+        if i < n:
+            new[i] = 3
+    new[min(700, n // 2)] = 700 if not two else 3000
+    pads = set(r.sample(range(2, n - 2), n // 8)) - {638, 639, 640, 1279, 1280, min(700, n // 2)}
+    lens = [c + r.choice((0, 0, 1, 30)) for c in new]
+    cache = _build(capi, "f16", lens, kv_heads, d, page, 3)
+    seqs = [-1 if i in pads else i for i in range(n)]
+    cu = [0]
+    for c in new:
+        cu.append(cu[-1] + c)
+    M = cu[-1] + 1
+    q = torch.randn((M, heads * d), device="cuda")
+    live = torch.zeros(M, dtype=torch.bool)
+    for i, s in enumerate(seqs):
+        if s != -1:
+            live[cu[i] : cu[i + 1]] = True
+    live = live.cuda()
+    bad = next(i for i in range(n // 3, n) if seqs[i] != -1 and new[i] > 0 and new[i] < 6)
+    for unsound in (None, n + 5):
+        listed = list(seqs)
+        if unsound is not None:
+            listed[bad] = unsound
+        out = torch.full_like(q, 3.25)
+        ctx.attn_prompt(cache, 0, q, _t(listed), _t(cu), 0.125, out=out)
+        if unsound is None:
+            ctx.sync()
+        else:
+            with pytest.raises(capi.NhbError) as e:
+                ctx.sync()
+            assert e.value.code == capi.ERR_ARG
+            listed[bad] = -1  # its rows stay as they are, like padding
+            live[cu[bad] : cu[bad + 1]] = False
+        _check_rows(cache, q.reshape(M, heads, d), out.reshape(M, heads, d), listed, cu, 0.125, "f16", what=(n, unsound))
+        assert (out[~live] == 3.25).all()
+
+
+@pytest.mark.parametrize("kind, d, page, heads, kv_heads", [("f16", 128, 64, 32, 8), ("bf16", 128, 32, 6, 2), ("f16", 64, 16, 7, 1), ("bf16", 64, 128, 4, 4)])
+def test_a_few_rows_behind_a_long_context(capi, ctx, kind, d, page, heads, kv_heads):
+    """Drafts to be verified, and a short turn, behind thousands of cached tokens."""
+    import torch
+
+    lens = [(9000, 4), (4321, 1), (2500, 16), (6001, 7)]
+    cache = _build(capi, kind, [a + b for a, b in lens], kv_heads, d, page, d + page)
+    cu = [0, 4, 5, 21, 28]
+    q = torch.randn((28, heads * d), device="cuda") * 1.5
+    scale = 1.0 / math.sqrt(d)
+    out = ctx.attn_prompt(cache, 0, q, _t([0, 1, 2, 3]), _t(cu), scale)
+    ctx.sync()
+    _check_rows(cache, q.reshape(28, heads, d), out.reshape(28, heads, d), [0, 1, 2, 3], cu, scale, kind)
+
+
+def test_append_finds_its_entry_in_a_long_list(capi, ctx):
+    """600 list entries (the search goes round beyond 256), one row each, none, or many; a CTA takes one token."""
+    import torch
+
+    r = random.Random(5)
+    n, d, kv_heads, heads, page = 600, 64, 2, 3, 16
+    new = [r.choice((0, 1, 1, 2, 19)) for _ in range(n)]
+    for i in (0, 255, 256, 257, 511, 512, n - 1):
+        new[i] = 2
+    seqs = r.sample(range(n), n)
+    for i in r.sample(range(1, n - 1), 40):
+        if i not in (255, 256, 257, 511, 512):
+            seqs[i] = -1
+    cu = np.concatenate([[0], np.cumsum(new)]).tolist()
+    M = cu[-1] + 2
+    cache = capi.KvCache.empty(1, 2 * n + 100, kv_heads, d, n, 64, page)
+    ctx.kv_reserve(cache, _t(seqs), _t(cu))
+    q, k, v = (torch.randn((M, h * d), device="cuda") for h in (heads, kv_heads, kv_heads))
+    out = ctx.rope_kv_append(cache, 0, q, k, v, _t(seqs), _t(cu), capi.Rope(1e4), q_out=torch.full_like(q, 4.0))
+    ctx.sync()
+    entry = [(i, t - cu[i]) for i in range(n) for t in range(cu[i], cu[i + 1])]
+    live = torch.tensor([seqs[i] != -1 for i, _ in entry] + [False, False]).cuda()
+    pos = torch.tensor([p for i, p in entry if seqs[i] != -1]).cuda()
+    which = torch.tensor([seqs[i] for i, p in entry if seqs[i] != -1]).cuda()
+    turn = lambda x, h: kv_model.rotate(x[live].reshape(-1, h, d), pos, 1e4, "pairs", d)  # noqa: E731
+    assert (out[live].double() - turn(q, heads).reshape(len(pos), -1)).abs().max().item() <= 10 * 2.0**-21 and (out[~live] == 4.0).all()
+    ids = cache.table[which, pos // page].long()
+    got_k, got_v = cache.k[0][ids, :, pos % page].double(), cache.v[0][ids, :, pos % page].double()
+    want_k, want_v = turn(k, kv_heads), v[live].reshape(-1, kv_heads, d).double()
+    assert ((got_k - want_k).abs() <= want_k.abs() * 2.0**-11 + 10 * 2.0**-21).all() and ((got_v - want_v).abs() <= want_v.abs() * 2.0**-11 + 2.0**-25).all()
+
+
 # ---- streams ----
 
 
