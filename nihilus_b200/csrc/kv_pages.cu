@@ -475,7 +475,7 @@ namespace nhb {
 		if (cache->page_tokens != 16 && cache->page_tokens != 32 && cache->page_tokens != 64 && cache->page_tokens != 128)
 			return fail(ctx, NHB_ERR_UNSUPPORTED, w + ": page_tokens must be 16, 32, 64 or 128");
 		if (cache->n_layers < 1 || cache->n_layers > 65536 || cache->n_pages < 1 || cache->n_pages > NHB_KV_MAX_PAGES || cache->kv_heads < 1 || cache->kv_heads > 1024 ||
-			cache->max_seqs < 1 || cache->max_seqs > NHB_KV_MAX_SEQS || cache->max_pages < 1 || cache->max_pages * cache->page_tokens > (int64_t(1) << 30))
+			cache->max_seqs < 1 || cache->max_seqs > NHB_KV_MAX_SEQS || cache->max_pages < 1 || cache->max_pages > (int64_t(1) << 30) / cache->page_tokens)
 			return fail(ctx, NHB_ERR_ARG, w + ": a size of the cache is out of range (layers and sequences up to 65536, pages up to 2^24, kv heads up to 1024, 2^30 tokens per sequence)");
 		if (cache->n_pages * cache->kv_heads * cache->page_tokens > INT32_MAX)
 			return fail(ctx, NHB_ERR_UNSUPPORTED, w + ": more than 2^31 - 1 rows (pages x kv heads x page_tokens) in a layer");

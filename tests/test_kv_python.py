@@ -193,3 +193,16 @@ def test_the_tensors_of_a_cache_cannot_be_replaced(capi):
             setattr(cache, name, t.clone())
         assert getattr(cache, name) is t
     cache.note = 1
+
+
+def test_a_table_whose_size_overflows_is_refused(capi):
+    """2^60 pages of 16 tokens are 2^64 tokens, which 64 bits take for none."""
+    import ctypes as C
+
+    p = 1 << 20
+    for max_pages, page in ((1 << 60, 16), ((1 << 60) + 5, 16), (1 << 57, 128), ((1 << 23) + 1, 128), (1 << 62, 64)):
+        struct = capi.KvCacheStruct(p, 2 * p, 3 * p, 4 * p, 5 * p, 1, 8, 2, page, 64, 4, max_pages, 0)
+        rc = capi.lib.nhb_kv_free(None, C.byref(struct), p, 1)
+        assert rc == capi.ERR_ARG and "out of range" in capi.last_error(), (max_pages, page, capi.last_error())
+    struct = capi.KvCacheStruct(p, 2 * p, 3 * p, 4 * p, 5 * p, 1, 8, 2, 128, 64, 4, 1 << 23, 0)
+    assert capi.lib.nhb_kv_free(None, C.byref(struct), p, 1) == capi.ERR_ARG and "null context" in capi.last_error()
