@@ -345,3 +345,35 @@ def test_new_outputs_of_a_context_on_another_stream(capi):
                 ctx.sync()
                 torch.cuda.synchronize()
                 assert torch.equal(got, ref) and (got != 0).any()
+
+
+def test_graphs_and_eager_calls_on_streams_in_turn(capi):
+    """One workspace: replays of two graphs and eager calls, each on another stream than the one before, none of them waited for."""
+    import torch
+
+    cache = _build(capi, "f16", [5000, 3000, 100], 8, 128, 64, 2)
+    q = torch.randn((3, 32 * 128), device="cuda")
+    seqs, fewer = _t([0, 1, 2]), _t([1, 2, 0])
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    ref, other, a, b, c = (torch.zeros_like(q) for _ in range(5))
+    torch.cuda.synchronize()
+    with capi.Context(0) as ctx:
+        ctx.attn_decode(cache, 0, q, seqs, 0.09, out=ref)
+        ctx.attn_decode(cache, 0, q, fewer, 0.09, out=other)
+        ctx.sync()
+        graphs = []
+        for which, out in ((seqs, a), (fewer, b)):
+            ctx.graph_begin()
+            ctx.attn_decode(cache, 0, q, which, 0.09, out=out)
+            graphs.append(ctx.graph_end())
+        for i in range(30):
+            ctx.set_stream(streams[i % 3].cuda_stream)
+            if i % 4 == 3:
+                ctx.attn_decode(cache, 0, q, seqs, 0.09, out=c)
+            else:
+                graphs[i % 2].launch()
+        ctx.sync()
+        torch.cuda.synchronize()
+        assert torch.equal(a, ref) and torch.equal(b, other) and torch.equal(c, ref)
+        for g in graphs:
+            g.free()
