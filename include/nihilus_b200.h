@@ -270,16 +270,20 @@ int nhb_rope_kv_append(nhb_ctx* ctx, const nhb_kv_cache* cache, int64_t layer, c
 /* ---- attention over the cache ----
  * out row = sum over keys j of softmax_j(scale * q . k_j) v_j, per head; query heads g * kv_head .. share kv_head (heads a multiple of
  * kv_heads).  Rows f32; q and out must not overlap.  Computed to f32 accuracy although the cache holds 16 bits: queries and
- * weights enter the tensor cores as two (f16) or three (bf16) 16-bit parts each.  scale > 0.  A row without keys becomes 0; keys past a sequence's
+ * weights enter the tensor cores as two (f16) or three (bf16) 16-bit parts each (of a bf16 cache: as long as q . k and the sum of
+ * a row's keys times |v| stay in the range of f32).  scale > 0.  A row without keys becomes 0; keys past a sequence's
  * length and keys a row may not see have no influence, whatever they hold; a row that sees a NaN key becomes NaN, one that sees
  * an infinite key NaN or, where its score is -inf, the value without that key (infinities and NaN in v reach the
  * columns they stand in).  Rows of padding entries and behind the last sequence stay as they are. */
 /* Prompts: row r of list entry i (see cu_dev) is the token at position lens[s] - (cu[i + 1] - cu[i]) + r - cu[i] and sees the keys up to
- * its own position, so a prompt may also continue what the cache already holds. */
+ * its own position, so a prompt may also continue what the cache already holds.  The keys of a row are not dealt to several SMs:
+ * few rows behind a long context (drafts, a short turn) take a time that grows with the context, 256 us for 4 rows behind 16000
+ * tokens on a B200.  Offsets that let two entries claim the same rows are reported where they make more tiles than M rows have. */
 int nhb_attn_prompt(nhb_ctx* ctx, const nhb_kv_cache* cache, int64_t layer, const float* q_dev, int64_t ldq, int64_t heads, int64_t M, const int32_t* seqs_dev,
 	const int32_t* cu_dev, int64_t n, float scale, float* out_dev, int64_t ldo);
 /* One token each: row i sees all lens[s] keys of sequence seqs[i].  shared: the first `shared` tokens of every sequence of the
- * list are the same tokens in the same pages (as nhb_kv_fork leaves them); their whole pages are read once for the batch.  A
+ * list are the same tokens in the same pages (as nhb_kv_fork leaves them); their whole pages are read once for the batch, by launches of
+ * their own: pass 0 where they are few (on a B200 it pays from about 1000 tokens for 64 sequences, from 6000 for 8).  A
  * sequence whose pages differ from those of the first entry is reported by nhb_sync (NHB_ERR_ARG).  0: nothing is shared. */
 int nhb_attn_decode(nhb_ctx* ctx, const nhb_kv_cache* cache, int64_t layer, const float* q_dev, int64_t ldq, int64_t heads, const int32_t* seqs_dev, int64_t n,
 	int64_t shared, float scale, float* out_dev, int64_t ldo);

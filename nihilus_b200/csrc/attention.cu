@@ -56,7 +56,8 @@ namespace nhb {
 				return launch_attn_prompt(ctx, c, a);
 			}
 			// what the batch shares is read once, by its own launch, whose partial results the decode kernel joins.  One sequence
-			// shares with nobody.
+			// shares with nobody.  (Worth its launches for long prefixes only, which is left to the caller.  bf16, up to 700 keys of their own, with
+			// the launches / with shared = 0: 64 sequences behind 12288 tokens 106 / 483 us, 1024 74 / 70, 512 74 / 52; 8 behind 12288 49 / 70, 4096 39 / 33.)
 			attn_prefix pre{};
 			prefix_plan plan{};
 			const bool prefix = a.shared_pages > 0 && a.n > 1;

@@ -20,10 +20,13 @@
 // Every wait is bounded; one that runs out is recorded for the host.  A warp whose wait ran out arrives nowhere any more, so that what waits for
 // it stops too, and the block ends only after its copies and products.
 //
-// B200, f16, 32 heads of 128 on 8: 8192 tokens 863 us (637 TFLOP/s of the formula, 1274 on the tensor cores; about 1.0 ms once the
-// power limit has brought the clock down), 2048 tokens 96 us, 77 tokens 15.5 us.  A step (one chain's scores and P V, 32
+// B200, f16, 32 heads of 128 on 8: 8192 tokens 1017 us (541 TFLOP/s of the formula, 1082 on the tensor cores; 890 in a burst, before the
+// power limit brings the clock down), 2048 tokens 94 us, 77 tokens 16 us.  A step (one chain's scores and P V, 32
 // m128n128k16) takes 2950 cycles of which the tensor cores need 2070; what is left is a chain's own way round: 2300 cycles of
-// softmax beside the other chain's, 1030 of P V, 900 to take the product.
+// softmax beside the other chain's, 1030 of P V, 900 to take the product.  The compiler spills: a warp and step make 10 loads and 3 stores of
+// local memory (counted: 1.40 M loads for 16896 steps).
+// The grid is row tiles x kv heads and a CTA walks all keys of its rows, so a few rows behind a long context leave most SMs idle: 4 rows behind
+// 16000 cached tokens take 256 us where a decode step of that sequence takes 21, and the time grows with the context.
 #include <algorithm>
 
 #include "attention.h"
