@@ -206,3 +206,18 @@ def test_a_table_whose_size_overflows_is_refused(capi):
         assert rc == capi.ERR_ARG and "out of range" in capi.last_error(), (max_pages, page, capi.last_error())
     struct = capi.KvCacheStruct(p, 2 * p, 3 * p, 4 * p, 5 * p, 1, 8, 2, 128, 64, 4, 1 << 23, 0)
     assert capi.lib.nhb_kv_free(None, C.byref(struct), p, 1) == capi.ERR_ARG and "null context" in capi.last_error()
+
+
+def test_torchs_stream_is_that_of_the_contexts_gpu(capi, monkeypatch):
+    """Asked for by the context's own device, whatever device is current; the same stream is not set twice."""
+    current = {0: 0, 1: 7777}
+    monkeypatch.setattr(capi, "_current_stream", current.__getitem__)
+    for device, handles in ((0, [1, 5555]), (1, [7777, 8888])):
+        ctx, sets = _context(capi), []
+        ctx.device = device
+        monkeypatch.setattr(ctx, "set_stream", lambda h, ctx=ctx, sets=sets: (sets.append(h), setattr(ctx, "stream", h)))
+        ctx.use_torch_stream()
+        ctx.use_torch_stream()
+        current[device] = handles[1]
+        ctx.use_torch_stream()
+        assert sets == handles
