@@ -247,7 +247,7 @@ int nhb_kv_fork(nhb_ctx* ctx, const nhb_kv_cache* cache, const int32_t* parents_
 /* The sequences end: their pages lose a reference each, lens = 0, table rows = -1.  Distinct sequences (else nothing changes). */
 int nhb_kv_free(nhb_ctx* ctx, const nhb_kv_cache* cache, const int32_t* seqs_dev, int64_t n);
 /* Closes the gaps: with L pages in use, those numbered L and above move, ascending, into the free ones below L, ascending, and every
- * table follows.  live_dev (device int32, may be NULL) receives L: pages from L on are free. */
+ * table follows.  live_dev (device int32, may be NULL) receives L: pages from L on are free.  A length that a table row cannot hold: nothing changes. */
 int nhb_kv_compact(nhb_ctx* ctx, const nhb_kv_cache* cache, int32_t* live_dev);
 
 /* ---- rotary embedding and the store into the cache ---- */

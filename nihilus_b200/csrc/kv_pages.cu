@@ -377,8 +377,17 @@ namespace nhb {
 			pdl_launch_dependents();
 			pdl_wait_prior_grids();
 			const plan_lists l = lists_at(ws, 0, c.n_pages);
-			const int live	   = collect(c.refs, 0, c.n_pages, false, nullptr, c.n_pages, scan);
-			__syncthreads();
+			bool bad		   = false;// a length that its table row cannot hold: the sequence's pages would move without it
+			for (int s = threadIdx.x; s < c.max_seqs; s += PLAN_THREADS)
+				bad = bad || c.lens[s] < 0 || c.lens[s] > kv_capacity(c);
+			const int live = collect(c.refs, 0, c.n_pages, false, nullptr, c.n_pages, scan);
+			if (__syncthreads_or(bad)) {
+				if (threadIdx.x == 0) {
+					l.head->copies = 0;
+					report(c.status, DEV_KV_BAD);
+				}
+				return;
+			}
 			// as many pages in use above `live` as free ones below it
 			const int moves = collect(c.refs, 0, live, true, l.dst, c.n_pages, scan);
 			__syncthreads();
@@ -410,10 +419,7 @@ namespace nhb {
 			const int live = __ldcg(&l.head->live);
 			const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, n_warps = (gridDim.x * blockDim.x) >> 5, lane = threadIdx.x & 31;
 			for (int s = warp; s < c.max_seqs; s += n_warps) {
-				const int tokens = c.lens[s];
-				if (tokens <= 0 || tokens > kv_capacity(c))
-					continue;
-				const int held = kv_pages_of(c, tokens);
+				const int held = kv_pages_of(c, c.lens[s]);
 				int* row	   = c.table + static_cast<size_t>(s) * c.max_pages;
 				for (int j = lane; j < held; j += 32) {
 					const int page = row[j];

@@ -377,3 +377,17 @@ def test_graphs_and_eager_calls_on_streams_in_turn(capi):
         assert torch.equal(a, ref) and torch.equal(b, other) and torch.equal(c, ref)
         for g in graphs:
             g.free()
+
+
+def test_compact_reports_a_length_it_cannot_follow(capi, ctx):
+    """The pages of such a sequence may move without its table: the caller has to know."""
+    cache = _build(capi, "f16", [40, 33, 16, 50], 1, 64, 16, 1, spare=6, max_tokens=64)
+    for length in (65, -1, 1 << 30):
+        cache.lens[1] = length
+        ctx.kv_compact(cache)
+        with pytest.raises(capi.NhbError) as e:
+            ctx.sync()
+        assert e.value.code == capi.ERR_ARG
+    cache.lens[1] = 0
+    ctx.kv_compact(cache)
+    ctx.sync()
