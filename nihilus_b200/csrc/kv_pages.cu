@@ -394,10 +394,10 @@ namespace nhb {
 			if (moves)
 				collect(c.refs, live, c.n_pages, false, l.src, moves, scan);
 			__syncthreads();
-			// rows: the new number of every page that moves, by its old one
+			// rows: which move a page takes part in, by its old number (what the others hold there is no move of theirs)
 			for (int i = threadIdx.x; i < moves; i += PLAN_THREADS) {
 				const int from = l.src[i], to = l.dst[i];
-				l.rows[from] = to;
+				l.rows[from] = i;
 				c.refs[to]	 = c.refs[from];
 				c.refs[from] = 0;
 			}
@@ -423,10 +423,15 @@ namespace nhb {
 				int* row	   = c.table + static_cast<size_t>(s) * c.max_pages;
 				for (int j = lane; j < held; j += 32) {
 					const int page = row[j];
-					if (page < 0 || page >= c.n_pages)
+					if (page < 0 || page >= c.n_pages) {
 						report(c.status, DEV_KV_BAD);
-					else if (page >= live)
-						row[j] = __ldcg(l.rows + page);
+					} else if (page >= live) {
+						const int move = __ldcg(l.rows + page);
+						if (move >= 0 && move < moves && __ldcg(l.src + move) == page)
+							row[j] = __ldcg(l.dst + move);
+						else
+							report(c.status, DEV_KV_BAD);// nobody counts the page
+					}
 				}
 			}
 			// whole pages: [kv_heads][page_tokens][head_dim] is one stretch of memory, moved in pieces of 4 KB

@@ -391,3 +391,21 @@ def test_compact_reports_a_length_it_cannot_follow(capi, ctx):
     cache.lens[1] = 0
     ctx.kv_compact(cache)
     ctx.sync()
+
+
+def test_compact_leaves_a_page_that_nobody_counts_where_it_is(capi, ctx):
+    """A table that holds a page whose count is zero, behind the pages in use: no move belongs to it.  It is reported and keeps its number."""
+    for behind in (1, 4):
+        cache = _build(capi, "f16", [40, 33, 16, 50], 1, 64, 16, 1, spare=6, max_tokens=64)
+        ctx.kv_free(cache, _t([0]))
+        ctx.kv_compact(cache)
+        ctx.sync()
+        page = int((cache.refs > 0).sum()) + behind  # free
+        cache.refs[cache.table[1, 0].long()] = 0
+        cache.table[1, 0] = page
+        others = cache.table[2:4].clone()
+        ctx.kv_compact(cache)  # one gap is closed by the last page in use
+        with pytest.raises(capi.NhbError) as e:
+            ctx.sync()
+        assert e.value.code == capi.ERR_ARG and cache.table[1, 0].item() == page
+        assert int((cache.table[2:4] != others).sum()) <= 1
